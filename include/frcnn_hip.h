@@ -360,6 +360,61 @@ int frcnn_resize_pad_f32(const float *src, int C, int in_h, int in_w, int out_h,
 int frcnn_resize_pad_batch_f32(const float *const *src_host, const int32_t *shape_host, int n, int C,
                                float *dst, int canvas_h, int canvas_w, void *stream);
 
+/* ---- 8-bit dense layers of the box head ---------------------------------------------------------
+ * The linear layers behind the RoI features (ROIHead/mlp_head.py:19-49, ROIHead/predictor.py:19-49; call site
+ * ROIHead/roi_head.py:132-135) on 8-bit integers with one scale for every row (RoI) and one for every output
+ * channel.  No counterpart in the reference, which runs them in fp32.
+ * Element types of `x`, `out` and the gradients: */
+#define FRCNN_F32 0
+#define FRCNN_BF16 1
+#define FRCNN_F16 2
+
+/* Row quantiser.  x: (M,K), row stride in elements (any, 0 for a broadcast row).  Per row: top = max |x|;
+ * scale = top / 127 in fp32; code = the whole number nearest to the exact quotient 127 x / top, ties to even (so in
+ * [-127, 127]).  A row of zeros has scale 0 and codes 0; a row with an Inf or a NaN has scale NaN and codes 0.
+ * n_rows: device int32 count of valid rows (clamped to [0, M]; rows behind it are neither read nor written) or NULL.
+ * codes: (M,K) bytes, row stride codes_stride >= K; with a stride that is a multiple of 16 (codes then 16-byte
+ * aligned) the bytes from K to the next multiple of 16 are written as zeros.  scale: (M). */
+int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows,
+                           int8_t *codes, int64_t codes_stride, float *scale, void *stream);
+
+/* out[m,n] = (sum_k a[m,k] b[n,k]) a_scale[m] b_scale[n] + bias[n], then max(., 0) if relu; NaN stays NaN.
+ * a: (M,K) bytes, b: (N,K) bytes, row strides in bytes (16-byte aligned rows are read in place, others are copied to
+ * the workspace first); K <= 131071: the 32-bit sums cannot wrap, whatever the bytes.  bias: (N) fp32 or NULL.  The
+ * sums are exact, scales and bias are applied in 64 bits, and the result is rounded to fp32 and then to out's type.
+ * n_rows as above: rows of out behind it are left as they were.  out: (M,N), row stride in elements.
+ * workspace: frcnn_matmul_i8_workspace_bytes(M,N,K) bytes, 256-byte aligned, contents need not survive. */
+size_t frcnn_matmul_i8_workspace_bytes(int M, int N, int K);
+int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b, int64_t b_stride,
+                    const float *b_scale, const float *bias, int relu, int M, int N, int K, const int32_t *n_rows,
+                    void *out, int out_type, int64_t out_stride, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* frcnn_quantize_rows_i8 on x and frcnn_matmul_i8 on its codes, which stay in the workspace
+ * (frcnn_linear_i8_workspace_bytes(M,N,K) bytes): one served layer in one call. */
+size_t frcnn_linear_i8_workspace_bytes(int M, int N, int K);
+int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, const int8_t *b, int64_t b_stride,
+                    const float *b_scale, const float *bias, int relu, int M, int N, int K, const int32_t *n_rows,
+                    void *out, int out_type, int64_t out_stride, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* Straight-through gradients of the layer (rounding counts as the identity), from grad = dL/dout (M,N) and the codes
+ * and scales of the forward call.  g = grad, or 0 where y <= 0 (y: the forward's output in grad's type if it ended in
+ * a ReLU, NULL otherwise):
+ *   grad_x[m,k] = sum_n g[m,n] b_scale[n] b[n,k]     grad_w[n,k] = sum_m g[m,n] a_scale[m] a[m,k]
+ *   grad_bias[n] = sum_m g[m,n]  (fp32, summed in a fixed order)
+ * The factors g b_scale and g a_scale are taken as 24-bit fixed-point numbers relative to the largest of their row m
+ * (grad_x) or column n (grad_w), and the sums over them are exact: an output is off by at most
+ * 2^-24 max|factor| sum|code| before its rounding.  An Inf or a NaN among a row's (column's) factors makes that whole
+ * row of grad_x (grad_w) NaN.  grad_x / grad_w: contiguous; grad_x, grad_w, grad_bias: NULL where not wanted.
+ * M, N, K <= 131071.  The results have the same bits every run. */
+size_t frcnn_linear_i8_backward_workspace_bytes(int M, int N, int K);
+int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t grad_stride, const void *y, int64_t y_stride,
+                             const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b,
+                             int64_t b_stride, const float *b_scale, int M, int N, int K, void *grad_x,
+                             int grad_x_type, void *grad_w, int grad_w_type, float *grad_bias, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

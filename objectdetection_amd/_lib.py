@@ -64,6 +64,14 @@ SIGNATURES = {
     "frcnn_roi_loss_f32": (_I, [_P, _P, _P, _P, _I, _I, _F, _P, _P, _P, _P]),
     "frcnn_resize_pad_f32": (_I, [_P, _I, _I, _I, _I, _I, _P, _I, _I, _P]),
     "frcnn_resize_pad_batch_f32": (_I, [_P, _P, _I, _I, _P, _I, _I, _P]),
+    "frcnn_quantize_rows_i8": (_I, [_P, _I, _L, _I, _I, _P, _P, _L, _P, _P]),
+    "frcnn_matmul_i8_workspace_bytes": (_Z, [_I, _I, _I]),
+    "frcnn_matmul_i8": (_I, [_P, _L, _P, _P, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _L, _P, _Z, _P]),
+    "frcnn_linear_i8_workspace_bytes": (_Z, [_I, _I, _I]),
+    "frcnn_linear_i8": (_I, [_P, _I, _L, _P, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _L, _P, _Z, _P]),
+    "frcnn_linear_i8_backward_workspace_bytes": (_Z, [_I, _I, _I]),
+    "frcnn_linear_i8_backward": (_I, [_P, _I, _L, _P, _L, _P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _I, _P, _I, _P, _P, _Z,
+                                      _P]),
 }
 
 

@@ -1,0 +1,461 @@
+// linear_i8.hip -- dense layers on 8-bit integers: out_mn = (sum_k a_mk b_nk) a_scale_m b_scale_n + bias_n, rows of a
+// (RoIs) and rows of b (output channels) both contiguous in k, and the two gradient products, which are the same
+// product on 24-bit fixed-point gradients (three 8-bit digits, three sums).
+//
+// The sums are exact: 32-bit integers cannot wrap below 2^17 products of two bytes.  Their order therefore does not
+// matter, and splitting k over workgroups changes no bit.  The scales and the bias are applied in 64 bits and the
+// result is rounded to fp32 (and from there to 16 bits): the sign a ReLU looks at is the sign of the exact expression.
+#include "i8_common.h"
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+#define LI_BK 128          // bytes of k per LDS stage
+#define LI_OOB 0x70000000  // a byte offset beyond every tile: the buffer load returns zeros unread
+#define LI_MAX_STRIDE 4000000 // 256 rows of it stay below LI_OOB
+
+struct LiArgs {
+    const int8_t *a, *b;
+    int64_t a_stride, b_stride, a_plane; // bytes
+    const int32_t *n_rows;               // device count of valid rows of a, or NULL
+    int M, N, K;
+    int tiles_m, tiles_n, k_split;       // k_split: bytes of k per split, a multiple of LI_BK
+    const float *a_scale, *b_scale, *bias;
+    int relu, out_type;
+    void *out;
+    int64_t out_stride;                  // elements
+    void *partial;                       // per-split sums, or NULL
+};
+
+// One result from an exact sum.  P = 3: a_scale is the magnitude that the digits are relative to.
+template <int P>
+__device__ __forceinline__ float li_finish(double sum, double a_scale, const LiArgs &A, int n)
+{
+    double z = sum * (P == 3 ? a_scale * (1.0 / (double)I8_FIX) : a_scale);
+    if (A.b_scale) z *= (double)A.b_scale[n];
+    if (A.bias) z += (double)A.bias[n];
+    if (A.relu) z = z < 0.0 ? 0.0 : z; // keeps NaN
+    return (float)z;
+}
+
+__device__ __forceinline__ void li_store1(const LiArgs &A, int64_t at, float z)
+{
+    if (A.out_type == FRCNN_F32) ((float *)A.out)[at] = z;
+    else if (A.out_type == FRCNN_BF16) ((__bf16 *)A.out)[at] = (__bf16)z;
+    else ((_Float16 *)A.out)[at] = (_Float16)z;
+}
+
+// Rows of 128 bytes in LDS; the 16-byte slot of chunk c of row r is c ^ li_swz(r): the rows a matrix instruction's lanes
+// read together (consecutive ones, or runs of four) then lie in different banks.
+__device__ __forceinline__ int li_swz(int r) { return (r ^ (r >> 2)) & 7; }
+
+template <int BM, int BN, int WM, int WN, int P>
+__device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
+{
+    constexpr int NW = (BM / WM) * (BN / WN);
+    constexpr int TM = WM / 16, TN = WN / 16;
+    constexpr int GA = BM / 8 / NW, GB = BN / 8 / NW; // loads (8 rows each) a wave issues per stage and plane
+    static_assert(GA * 8 * NW == BM && GB * 8 * NW == BN, "tile rows have to divide over the waves");
+    __shared__ __align__(1024) int8_t s0[(P * BM + BN) * LI_BK];
+    __shared__ __align__(1024) int8_t s1[(P * BM + BN) * LI_BK];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile_n = blockIdx.x % A.tiles_n, tile_m = blockIdx.x / A.tiles_n;
+    const int M = i8_rows(A.n_rows, A.M);
+    const int m0 = tile_m * BM, n0 = tile_n * BN;
+    if (m0 >= M) return;
+    const int ks = blockIdx.y * A.k_split;
+    const int ke = ks + A.k_split < A.K ? ks + A.k_split : A.K;
+    const int rows_a = M - m0 < BM ? M - m0 : BM, rows_b = A.N - n0 < BN ? A.N - n0 : BN;
+    const int kp = (A.K + 15) & ~15;
+
+    __amdgpu_buffer_rsrc_t ra[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+        ra[p] = __builtin_amdgcn_make_buffer_rsrc((void *)(A.a + p * A.a_plane + (int64_t)m0 * A.a_stride), 0,
+                                                  (int)((rows_a - 1) * A.a_stride) + kp, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(A.b + (int64_t)n0 * A.b_stride), 0, (int)((rows_b - 1) * A.b_stride) + kp, 0x00020000);
+    int va[GA], vb[GB], ca[GA], cb[GB];
+#pragma unroll
+    for (int j = 0; j < GA; ++j) {
+        const int r = (wave * GA + j) * 8 + (lane >> 3);
+        ca[j] = ((lane & 7) ^ li_swz(r)) * 16;
+        va[j] = r * (int)A.a_stride + ca[j];
+    }
+#pragma unroll
+    for (int j = 0; j < GB; ++j) {
+        const int r = (wave * GB + j) * 8 + (lane >> 3);
+        cb[j] = ((lane & 7) ^ li_swz(r)) * 16;
+        vb[j] = r * (int)A.b_stride + cb[j];
+    }
+    // one stage of LI_BK bytes of k: chunks at and beyond the end of k are not read (zeros)
+    auto fill = [&](int8_t *s, int k0) {
+#pragma unroll
+        for (int j = 0; j < GA; ++j) {
+            const int v = k0 + ca[j] < ke ? va[j] : LI_OOB;
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra[p], (lds_void *)(s + (p * BM + (wave * GA + j) * 8) * LI_BK), 16,
+                                                         v, k0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < GB; ++j) {
+            const int v = k0 + cb[j] < ke ? vb[j] : LI_OOB;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(s + (P * BM + (wave * GB + j) * 8) * LI_BK), 16, v, k0, 0,
+                                                     0);
+        }
+    };
+    // the last chunk of k may hold bytes of whatever follows the row: cleared in a's rows
+    auto clear_tail = [&](int8_t *s, int k0) {
+        if (k0 + LI_BK > A.K && (A.K & 15)) {
+            for (int r = threadIdx.x; r < P * BM; r += NW * 64) {
+                const int c = (A.K - k0) >> 4;
+                int8_t *q = s + r * LI_BK + ((c ^ li_swz(r % BM)) << 4);
+                for (int j = A.K & 15; j < 16; ++j) q[j] = 0;
+            }
+            __syncthreads();
+        }
+    };
+    const int wm0 = (wave % (BM / WM)) * WM, wn0 = (wave / (BM / WM)) * WN;
+    const int i16 = lane & 15, q4 = lane >> 4;
+    i32x4 acc[P][TM][TN];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn) acc[p][tm][tn] = (i32x4){0, 0, 0, 0};
+    // b is the instruction's row operand: a lane's four results are then neighbours in n, and with the rows of the TN
+    // tiles dealt out in fours a lane holds 4 TN of them
+    auto compute = [&](const int8_t *s) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            i32x4 fb[TN];
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn) {
+                const int r = wn0 + (i16 >> 2) * (4 * TN) + tn * 4 + (i16 & 3);
+                fb[tn] = *(const i32x4 *)(s + (P * BM + r) * LI_BK + (((kk * 4 + q4) ^ li_swz(r)) << 4));
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int tm = 0; tm < TM; ++tm) {
+                    const int r = wm0 + tm * 16 + i16;
+                    const i32x4 fa = *(const i32x4 *)(s + (p * BM + r) * LI_BK + (((kk * 4 + q4) ^ li_swz(r)) << 4));
+#pragma unroll
+                    for (int tn = 0; tn < TN; ++tn)
+                        acc[p][tm][tn] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[tn], fa, acc[p][tm][tn], 0, 0, 0);
+                }
+        }
+    };
+    fill(s0, ks);
+    for (int k0 = ks; k0 < ke; k0 += 2 * LI_BK) {
+        __syncthreads(); // s0 filled by every wave, s1 read by every wave
+        fill(s1, k0 + LI_BK);
+        clear_tail(s0, k0);
+        compute(s0);
+        if (k0 + LI_BK >= ke) break;
+        __syncthreads();
+        fill(s0, k0 + 2 * LI_BK);
+        clear_tail(s1, k0 + LI_BK);
+        compute(s1);
+    }
+
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+        const int m = m0 + wm0 + tm * 16 + i16;
+        if (m >= M) continue;
+        const double sa = A.partial ? 0.0 : (double)A.a_scale[m];
+#pragma unroll
+        for (int tn = 0; tn < TN; ++tn)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + wn0 + q4 * (4 * TN) + tn * 4 + r;
+                if (n >= A.N) continue;
+                if (A.partial) {
+                    const int64_t at = ((int64_t)blockIdx.y * A.M + m) * A.N + n;
+                    if (P == 1) ((int32_t *)A.partial)[at] = acc[0][tm][tn][r];
+                    else
+                        ((int64_t *)A.partial)[at] = ((int64_t)acc[0][tm][tn][r] << 16) +
+                                                     ((int64_t)acc[P > 1 ? 1 : 0][tm][tn][r] << 8) + acc[P > 2 ? 2 : 0][tm][tn][r];
+                } else {
+                    double s = (double)acc[0][tm][tn][r];
+                    if (P == 3)
+                        s = s * 65536.0 + (double)acc[P > 1 ? 1 : 0][tm][tn][r] * 256.0 + (double)acc[P > 2 ? 2 : 0][tm][tn][r];
+                    li_store1(A, (int64_t)m * A.out_stride + n, li_finish<P>(s, sa, A, n));
+                }
+            }
+    }
+}
+
+// (The body is a device function: a kernel template with these builtins in it is dropped from the host pass.)
+template <int BM, int BN, int WM, int WN, int P>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64)
+linear_i8_kernel(const LiArgs A)
+{
+    linear_i8_tile<BM, BN, WM, WN, P>(A);
+}
+
+// Joins the sums of a split k.
+template <int P>
+__global__ void __launch_bounds__(256)
+linear_i8_join_kernel(const LiArgs A, int splits)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t MN = (int64_t)A.M * A.N;
+    if (i >= MN) return;
+    const int m = (int)(i / A.N), n = (int)(i - (int64_t)m * A.N);
+    if (m >= i8_rows(A.n_rows, A.M)) return;
+    double s;
+    if (P == 1) {
+        int32_t t = 0;
+        for (int k = 0; k < splits; ++k) t += ((const int32_t *)A.partial)[k * MN + i];
+        s = (double)t;
+    } else {
+        int64_t t = 0;
+        for (int k = 0; k < splits; ++k) t += ((const int64_t *)A.partial)[k * MN + i];
+        s = (double)t;
+    }
+    li_store1(A, (int64_t)m * A.out_stride + n, li_finish<P>(s, (double)A.a_scale[m], A, n));
+}
+
+static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+struct LiPlan {
+    int bm, bn, splits, k_split;
+};
+
+// Tile by the rows there are; k is split until about every CU has a workgroup, down to 512 bytes each.
+static LiPlan li_plan(int M, int N, int K, int P)
+{
+    LiPlan p;
+    p.bm = p.bn = 64;
+    if (P == 1 && M <= 32) p.bm = 32;
+    else if (M > 64 && N > 64) p.bm = p.bn = 128;
+    const int64_t tiles = (int64_t)((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
+    const int steps = (K + LI_BK - 1) / LI_BK;
+    int64_t want = tiles >= 256 ? 1 : 256 / tiles;
+    const int most = steps / 4 > 0 ? steps / 4 : 1;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    const int per = (steps + (int)want - 1) / (int)want;
+    p.k_split = per * LI_BK;
+    p.splits = (steps + per - 1) / per;
+    return p;
+}
+
+static size_t li_partial_bytes(const LiPlan &p, int M, int N, int P)
+{
+    return p.splits > 1 ? up256((size_t)p.splits * M * N * (P == 3 ? 8 : 4)) : 0;
+}
+
+template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *partial, hipStream_t st)
+{
+    A.tiles_m = (A.M + p.bm - 1) / p.bm;
+    A.tiles_n = (A.N + p.bn - 1) / p.bn;
+    A.k_split = p.k_split;
+    A.partial = p.splits > 1 ? partial : nullptr;
+    const int64_t tiles = (int64_t)A.tiles_m * A.tiles_n;
+    FRCNN_REQUIRE(tiles < (1ll << 31), "linear_i8: too many tiles");
+    const dim3 grid((unsigned)tiles, p.splits);
+    if (p.bm == 128) {
+        if (P == 1) hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 64, 1>), grid, dim3(256), 0, st, A);
+        else hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 32, 3>), grid, dim3(512), 0, st, A);
+    } else if (p.bm == 64) {
+        hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, P>), grid, dim3(256), 0, st, A);
+    } else {
+        hipLaunchKernelGGL((linear_i8_kernel<32, 64, 16, 32, 1>), grid, dim3(256), 0, st, A);
+    }
+    FRCNN_CHECK_LAUNCH("linear_i8");
+    if (p.splits > 1) {
+        const int64_t MN = (int64_t)A.M * A.N;
+        hipLaunchKernelGGL((linear_i8_join_kernel<P>), dim3((unsigned)((MN + 255) / 256)), dim3(256), 0, st, A, p.splits);
+        FRCNN_CHECK_LAUNCH("linear_i8_join");
+    }
+    return FRCNN_OK;
+}
+
+// ---- entry points ------------------------------------------------------------------------------------------------------
+static int64_t li_stride(int K) { return ((int64_t)K + 15) / 16 * 16; }
+
+// Rows that the kernel reads in place: 16-byte aligned, and not overlapping.  (The last chunk of a row may reach up to 15
+// bytes beyond K; it is aligned like the row's start, so it lies in the same 16 bytes as the row's last element.)
+static bool li_in_place(const void *p, int64_t stride, int K)
+{
+    return ((uintptr_t)p & 15) == 0 && (stride & 15) == 0 && stride >= K && stride <= LI_MAX_STRIDE;
+}
+
+static bool li_shape_ok(int M, int N, int K) { return M >= 0 && N > 0 && K > 0 && K <= I8_MAX_K && (int64_t)M * N < (1ll << 40); }
+
+extern "C" size_t frcnn_matmul_i8_workspace_bytes(int M, int N, int K)
+{
+    if (!li_shape_ok(M, N, K) || M == 0) return 0;
+    // rows of a and b copied to an aligned stride where the caller's are not, and the sums of a split k
+    return up256((size_t)M * li_stride(K)) + up256((size_t)N * li_stride(K)) + li_partial_bytes(li_plan(M, N, K, 1), M, N, 1);
+}
+
+extern "C" int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b, int64_t b_stride,
+                               const float *b_scale, const float *bias, int relu, int M, int N, int K,
+                               const int32_t *n_rows, void *out, int out_type, int64_t out_stride, void *workspace,
+                               size_t workspace_bytes, void *stream)
+{
+    FRCNN_REQUIRE(li_shape_ok(M, N, K), "matmul_i8: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(i8_type_ok(out_type), "matmul_i8: unknown element type %d", out_type);
+    FRCNN_REQUIRE(a_stride >= 0 && b_stride >= 0 && out_stride >= N, "matmul_i8: bad strides");
+    if (M == 0) return FRCNN_OK;
+    FRCNN_REQUIRE(a && a_scale && b && b_scale && out, "matmul_i8: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    const LiPlan p = li_plan(M, N, K, 1);
+    char *ws = (char *)workspace;
+    const size_t need = frcnn_matmul_i8_workspace_bytes(M, N, K);
+    if (workspace_bytes < need || (need && !workspace)) {
+        frcnn_set_error("matmul_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
+        return FRCNN_EWORKSPACE;
+    }
+    const int64_t ld = li_stride(K);
+    LiArgs A = {};
+    if (M == 1) a_stride = ld;
+    if (li_in_place(a, a_stride, K)) {
+        A.a = a;
+        A.a_stride = a_stride;
+    } else {
+        int rc = frcnn_i8_pad_rows(a, a_stride, M, K, (int8_t *)ws, ld, st);
+        if (rc != FRCNN_OK) return rc;
+        A.a = (const int8_t *)ws;
+        A.a_stride = ld;
+    }
+    ws += up256((size_t)M * ld);
+    if (N == 1) b_stride = ld;
+    if (li_in_place(b, b_stride, K)) {
+        A.b = b;
+        A.b_stride = b_stride;
+    } else {
+        int rc = frcnn_i8_pad_rows(b, b_stride, N, K, (int8_t *)ws, ld, st);
+        if (rc != FRCNN_OK) return rc;
+        A.b = (const int8_t *)ws;
+        A.b_stride = ld;
+    }
+    ws += up256((size_t)N * ld);
+    A.n_rows = n_rows;
+    A.M = M; A.N = N; A.K = K;
+    A.a_scale = a_scale; A.b_scale = b_scale; A.bias = bias;
+    A.relu = relu; A.out_type = out_type; A.out = out; A.out_stride = out_stride;
+    return li_launch<1>(A, p, ws, st);
+}
+
+extern "C" size_t frcnn_linear_i8_workspace_bytes(int M, int N, int K)
+{
+    if (!li_shape_ok(M, N, K) || M == 0) return 0;
+    return up256((size_t)M * 4) + up256((size_t)M * li_stride(K)) + frcnn_matmul_i8_workspace_bytes(M, N, K);
+}
+
+extern "C" int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, const int8_t *b, int64_t b_stride,
+                               const float *b_scale, const float *bias, int relu, int M, int N, int K,
+                               const int32_t *n_rows, void *out, int out_type, int64_t out_stride, void *workspace,
+                               size_t workspace_bytes, void *stream)
+{
+    FRCNN_REQUIRE(li_shape_ok(M, N, K), "linear_i8: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    if (M == 0) return FRCNN_OK;
+    const size_t need = frcnn_linear_i8_workspace_bytes(M, N, K);
+    if (workspace_bytes < need || !workspace) {
+        frcnn_set_error("linear_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
+        return FRCNN_EWORKSPACE;
+    }
+    char *ws = (char *)workspace;
+    float *a_scale = (float *)ws;
+    int8_t *a = (int8_t *)(ws + up256((size_t)M * 4));
+    char *rest = (char *)a + up256((size_t)M * li_stride(K));
+    int rc = frcnn_quantize_rows_i8(x, x_type, x_stride, M, K, n_rows, a, li_stride(K), a_scale, stream);
+    if (rc != FRCNN_OK) return rc;
+    return frcnn_matmul_i8(a, li_stride(K), a_scale, b, b_stride, b_scale, bias, relu, M, N, K, n_rows, out, out_type,
+                           out_stride, rest, workspace_bytes - (size_t)(rest - ws), stream);
+}
+
+// Workspace of the gradients: for dL/dx the digits (3, M, N), their magnitudes, b transposed (K, N) and the sums of a
+// split; for dL/dw the digits (3, N, M), magnitudes, column partials, a transposed (K, M) and the sums of a split.
+struct LiGrad {
+    size_t digits, top, col_sum, partials, other, split, total;
+    LiPlan plan;
+};
+
+static LiGrad li_grad_plan(int rows, int cols, int inner, size_t partials)
+{ // a product (rows, cols) over `inner`
+    LiGrad g;
+    const size_t ld = (size_t)li_stride(inner);
+    size_t off = 0;
+    g.plan = li_plan(rows, cols, inner, 3);
+    g.digits = off; off += up256(3 * (size_t)rows * ld);
+    g.top = off; off += up256((size_t)rows * 4);
+    g.col_sum = off; off += up256((size_t)rows * 4);
+    g.partials = off; off += up256(partials);
+    g.other = off; off += up256((size_t)cols * ld);
+    g.split = off; off += li_partial_bytes(g.plan, rows, cols, 3);
+    g.total = off;
+    return g;
+}
+
+extern "C" size_t frcnn_linear_i8_backward_workspace_bytes(int M, int N, int K)
+{
+    if (M <= 0 || N <= 0 || K <= 0 || M > I8_MAX_K || N > I8_MAX_K || K > I8_MAX_K) return 0;
+    const size_t x = li_grad_plan(M, K, N, 0).total, w = li_grad_plan(N, K, M, frcnn_i8_grad_col_partials(M, N)).total;
+    return x > w ? x : w;
+}
+
+extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t grad_stride, const void *y,
+                                        int64_t y_stride, const int8_t *a, int64_t a_stride, const float *a_scale,
+                                        const int8_t *b, int64_t b_stride, const float *b_scale, int M, int N, int K,
+                                        void *grad_x, int grad_x_type, void *grad_w, int grad_w_type, float *grad_bias,
+                                        void *workspace, size_t workspace_bytes, void *stream)
+{
+    FRCNN_REQUIRE(M > 0 && N > 0 && K > 0 && M <= I8_MAX_K && N <= I8_MAX_K && K <= I8_MAX_K,
+                  "linear_i8_backward: bad shape (%d, %d, %d); each is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(i8_type_ok(grad_type) && i8_type_ok(grad_x_type) && i8_type_ok(grad_w_type),
+                  "linear_i8_backward: unknown element type");
+    FRCNN_REQUIRE(grad && a && a_scale && b && b_scale, "linear_i8_backward: null pointer");
+    FRCNN_REQUIRE(grad_stride >= 0 && y_stride >= 0 && a_stride >= 0 && b_stride >= 0, "linear_i8_backward: bad strides");
+    const size_t need = frcnn_linear_i8_backward_workspace_bytes(M, N, K);
+    if (workspace_bytes < need || !workspace) {
+        frcnn_set_error("linear_i8_backward: workspace too small (%zu < %zu)", workspace_bytes, need);
+        return FRCNN_EWORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    char *ws = (char *)workspace;
+    if (grad_x) {
+        const LiGrad g = li_grad_plan(M, K, N, 0);
+        const int64_t ld = li_stride(N), plane = (int64_t)M * ld;
+        int rc = frcnn_i8_grad_row_digits(grad, grad_type, grad_stride, y, y_stride, b_scale, M, N, (int8_t *)(ws + g.digits),
+                                          ld, plane, (float *)(ws + g.top), st);
+        if (rc != FRCNN_OK) return rc;
+        rc = frcnn_i8_transpose(b, b_stride, N, K, (int8_t *)(ws + g.other), ld, st);
+        if (rc != FRCNN_OK) return rc;
+        LiArgs A = {};
+        A.a = (const int8_t *)(ws + g.digits); A.a_stride = ld; A.a_plane = plane;
+        A.b = (const int8_t *)(ws + g.other); A.b_stride = ld;
+        A.M = M; A.N = K; A.K = N;
+        A.a_scale = (const float *)(ws + g.top);
+        A.out = grad_x; A.out_type = grad_x_type; A.out_stride = K;
+        rc = li_launch<3>(A, g.plan, ws + g.split, st);
+        if (rc != FRCNN_OK) return rc;
+    }
+    if (grad_w || grad_bias) { // the bias gradient is a by-product of the columns' magnitudes
+        const LiGrad g = li_grad_plan(N, K, M, frcnn_i8_grad_col_partials(M, N));
+        const int64_t ld = li_stride(M), plane = (int64_t)N * ld;
+        int rc = frcnn_i8_grad_col_digits(grad, grad_type, grad_stride, y, y_stride, a_scale, M, N, (int8_t *)(ws + g.digits),
+                                          ld, plane, (float *)(ws + g.top), grad_bias, ws + g.partials, st);
+        if (rc != FRCNN_OK) return rc;
+        if (!grad_w) return FRCNN_OK;
+        rc = frcnn_i8_transpose(a, a_stride, M, K, (int8_t *)(ws + g.other), ld, st);
+        if (rc != FRCNN_OK) return rc;
+        LiArgs A = {};
+        A.a = (const int8_t *)(ws + g.digits); A.a_stride = ld; A.a_plane = plane;
+        A.b = (const int8_t *)(ws + g.other); A.b_stride = ld;
+        A.M = N; A.N = K; A.K = M;
+        A.a_scale = (const float *)(ws + g.top);
+        A.out = grad_w; A.out_type = grad_w_type; A.out_stride = K;
+        rc = li_launch<3>(A, g.plan, ws + g.split, st);
+        if (rc != FRCNN_OK) return rc;
+    }
+    return FRCNN_OK;
+}
