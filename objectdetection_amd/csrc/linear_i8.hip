@@ -45,23 +45,59 @@ __device__ __forceinline__ void li_store1(const LiArgs &A, int64_t at, float z)
     else ((_Float16 *)A.out)[at] = (_Float16)z;
 }
 
-// Rows of 128 bytes in LDS; the 16-byte slot of chunk c of row r is c ^ li_swz(r): the rows a matrix instruction's lanes
-// read together (consecutive ones, or runs of four) then lie in different banks.
-__device__ __forceinline__ int li_swz(int r) { return (r ^ (r >> 2)) & 7; }
+// Four neighbours; the address is aligned to one element.
+__device__ __forceinline__ void li_store4(const LiArgs &A, int64_t at, const float (&z)[4])
+{
+    if (A.out_type == FRCNN_F32) {
+        __builtin_memcpy((float *)A.out + at, z, 16);
+    } else if (A.out_type == FRCNN_BF16) {
+        const __bf16 h[4] = {(__bf16)z[0], (__bf16)z[1], (__bf16)z[2], (__bf16)z[3]};
+        __builtin_memcpy((__bf16 *)A.out + at, h, 8);
+    } else {
+        const _Float16 h[4] = {(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]};
+        __builtin_memcpy((_Float16 *)A.out + at, h, 8);
+    }
+}
 
-template <int BM, int BN, int WM, int WN, int P>
+// A stage of LDS holds BK bytes of k for the tile's rows of a (P planes) and of b.  The 16-byte slot of chunk c of row r
+// is c ^ swizzle(r): sixteen consecutive rows, which the lanes of a matrix instruction read together, then cover all 64
+// banks once.
+template <int BK> __device__ __forceinline__ int li_swz(int r) { return BK == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+
+// Workgroups go to the eight XCDs in turn: neighbours in the tile order go to one XCD, eight tiles of m by all of n, so
+// that its L2 sees a row of a and a row of b several times.
+__device__ __forceinline__ void li_tile(int tiles_m, int tiles_n, int &tm, int &tn)
+{
+    const int tiles = tiles_m * tiles_n;
+    const int xcd = blockIdx.x & 7, q = tiles >> 3, r = tiles & 7;
+    const int l = xcd * q + (xcd < r ? xcd : r) + (blockIdx.x >> 3);
+    const int group = l / (8 * tiles_n), rem = l - group * 8 * tiles_n;
+    const int gm = tiles_m - group * 8 < 8 ? tiles_m - group * 8 : 8;
+    tm = group * 8 + rem % gm;
+    tn = rem / gm;
+}
+
+// One tile of BM x BN by waves of WM x WN, k in stages of BK bytes that travel global -> LDS directly, NST stages in
+// flight.
+template <int BM, int BN, int WM, int WN, int P, int BK, int NST>
 __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
 {
     constexpr int NW = (BM / WM) * (BN / WN);
     constexpr int TM = WM / 16, TN = WN / 16;
-    constexpr int GA = BM / 8 / NW, GB = BN / 8 / NW; // loads (8 rows each) a wave issues per stage and plane
-    static_assert(GA * 8 * NW == BM && GB * 8 * NW == BN, "tile rows have to divide over the waves");
-    __shared__ __align__(1024) int8_t s0[(P * BM + BN) * LI_BK];
-    __shared__ __align__(1024) int8_t s1[(P * BM + BN) * LI_BK];
+    constexpr int RPL = 1024 / BK, CPR = BK / 16; // rows a load of 64 x 16 bytes covers, chunks of a row
+    constexpr int GA = BM / RPL / NW, GB = BN / RPL / NW; // loads a wave issues per stage (and plane)
+    constexpr int LPS = GA * P + GB;
+    constexpr int STAGE = (P * BM + BN) * BK;
+    static_assert(GA * RPL * NW == BM && GB * RPL * NW == BN, "tile rows have to divide over the waves");
+    __shared__ __align__(1024) int8_t s0[STAGE];
+    __shared__ __align__(1024) int8_t s1[STAGE];
+    __shared__ __align__(1024) int8_t s2[NST > 2 ? STAGE : 16];
+    __shared__ __align__(1024) int8_t s3[NST > 3 ? STAGE : 16];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile_n = blockIdx.x % A.tiles_n, tile_m = blockIdx.x / A.tiles_n;
+    int tile_m, tile_n;
+    li_tile(A.tiles_m, A.tiles_n, tile_m, tile_n);
     const int M = i8_rows(A.n_rows, A.M);
     const int m0 = tile_m * BM, n0 = tile_n * BN;
     if (m0 >= M) return;
@@ -77,46 +113,47 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
                                                   (int)((rows_a - 1) * A.a_stride) + kp, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(A.b + (int64_t)n0 * A.b_stride), 0, (int)((rows_b - 1) * A.b_stride) + kp, 0x00020000);
-    int va[GA], vb[GB], ca[GA], cb[GB];
+    int va[GA], vb[GB];
+    // rows of one wave's loads are RPL apart, a multiple of the swizzle's period or not: the chunk is per load
+    int ca[GA], cb[GB];
 #pragma unroll
     for (int j = 0; j < GA; ++j) {
-        const int r = (wave * GA + j) * 8 + (lane >> 3);
-        ca[j] = ((lane & 7) ^ li_swz(r)) * 16;
+        const int r = (wave * GA + j) * RPL + lane / CPR;
+        ca[j] = ((lane % CPR) ^ li_swz<BK>(r)) * 16;
         va[j] = r * (int)A.a_stride + ca[j];
     }
 #pragma unroll
     for (int j = 0; j < GB; ++j) {
-        const int r = (wave * GB + j) * 8 + (lane >> 3);
-        cb[j] = ((lane & 7) ^ li_swz(r)) * 16;
+        const int r = (wave * GB + j) * RPL + lane / CPR;
+        cb[j] = ((lane % CPR) ^ li_swz<BK>(r)) * 16;
         vb[j] = r * (int)A.b_stride + cb[j];
     }
-    // one stage of LI_BK bytes of k: chunks at and beyond the end of k are not read (zeros)
+    // Chunks at and beyond the end of k are not read: their offset is beyond the buffer and the load stores zeros.  A
+    // stage past the end is filled like any other, so that the count of loads in flight is the same in every step.
     auto fill = [&](int8_t *s, int k0) {
 #pragma unroll
         for (int j = 0; j < GA; ++j) {
             const int v = k0 + ca[j] < ke ? va[j] : LI_OOB;
 #pragma unroll
             for (int p = 0; p < P; ++p)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra[p], (lds_void *)(s + (p * BM + (wave * GA + j) * 8) * LI_BK), 16,
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra[p], (lds_void *)(s + (p * BM + (wave * GA + j) * RPL) * BK), 16,
                                                          v, k0, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < GB; ++j) {
             const int v = k0 + cb[j] < ke ? vb[j] : LI_OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(s + (P * BM + (wave * GB + j) * 8) * LI_BK), 16, v, k0, 0,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(s + (P * BM + (wave * GB + j) * RPL) * BK), 16, v, k0, 0,
                                                      0);
         }
     };
     // the last chunk of k may hold bytes of whatever follows the row: cleared in a's rows
     auto clear_tail = [&](int8_t *s, int k0) {
-        if (k0 + LI_BK > A.K && (A.K & 15)) {
-            for (int r = threadIdx.x; r < P * BM; r += NW * 64) {
-                const int c = (A.K - k0) >> 4;
-                int8_t *q = s + r * LI_BK + ((c ^ li_swz(r % BM)) << 4);
-                for (int j = A.K & 15; j < 16; ++j) q[j] = 0;
-            }
-            __syncthreads();
+        for (int r = threadIdx.x; r < P * BM; r += NW * 64) {
+            const int c = (A.K - k0) >> 4;
+            int8_t *q = s + r * BK + ((c ^ li_swz<BK>(r % BM)) << 4);
+            for (int j = A.K & 15; j < 16; ++j) q[j] = 0;
         }
+        __syncthreads();
     };
     const int wm0 = (wave % (BM / WM)) * WM, wn0 = (wave / (BM / WM)) * WN;
     const int i16 = lane & 15, q4 = lane >> 4;
@@ -127,75 +164,126 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
         for (int tm = 0; tm < TM; ++tm)
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn) acc[p][tm][tn] = (i32x4){0, 0, 0, 0};
-    // b is the instruction's row operand: a lane's four results are then neighbours in n, and with the rows of the TN
-    // tiles dealt out in fours a lane holds 4 TN of them
+    // b is the instruction's row operand: a lane's four results are neighbours in n
+    const int swz = li_swz<BK>(i16);
     auto compute = [&](const int8_t *s) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
+        for (int kk = 0; kk < BK / 64; ++kk) {
+            const int at = i16 * BK + (((kk * 4 + q4) ^ swz) << 4);
             i32x4 fb[TN];
 #pragma unroll
-            for (int tn = 0; tn < TN; ++tn) {
-                const int r = wn0 + (i16 >> 2) * (4 * TN) + tn * 4 + (i16 & 3);
-                fb[tn] = *(const i32x4 *)(s + (P * BM + r) * LI_BK + (((kk * 4 + q4) ^ li_swz(r)) << 4));
-            }
+            for (int tn = 0; tn < TN; ++tn) fb[tn] = *(const i32x4 *)(s + (P * BM + wn0 + tn * 16) * BK + at);
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
                 for (int tm = 0; tm < TM; ++tm) {
-                    const int r = wm0 + tm * 16 + i16;
-                    const i32x4 fa = *(const i32x4 *)(s + (p * BM + r) * LI_BK + (((kk * 4 + q4) ^ li_swz(r)) << 4));
+                    const i32x4 fa = *(const i32x4 *)(s + (p * BM + wm0 + tm * 16) * BK + at);
 #pragma unroll
                     for (int tn = 0; tn < TN; ++tn)
                         acc[p][tm][tn] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[tn], fa, acc[p][tm][tn], 0, 0, 0);
                 }
         }
     };
+    // One step: this stage's loads are complete in this wave (the NST - 2 later stages may be in flight) and, behind the
+    // barrier, in all; every wave has read the previous stage (lgkmcnt), whose buffer the next fill overwrites.
+    auto step = [&](int8_t *cur, int8_t *next, int k0) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LPS * (NST - 2)) : "memory");
+        fill(next, k0 + (NST - 1) * BK);
+        if (k0 + BK > A.K && (A.K & 15)) clear_tail(cur, k0);
+        compute(cur);
+    };
     fill(s0, ks);
-    for (int k0 = ks; k0 < ke; k0 += 2 * LI_BK) {
-        __syncthreads(); // s0 filled by every wave, s1 read by every wave
-        fill(s1, k0 + LI_BK);
-        clear_tail(s0, k0);
-        compute(s0);
-        if (k0 + LI_BK >= ke) break;
-        __syncthreads();
-        fill(s0, k0 + 2 * LI_BK);
-        clear_tail(s1, k0 + LI_BK);
-        compute(s1);
+    if (NST > 2) fill(s1, ks + BK);
+    if (NST > 3) fill(s2, ks + 2 * BK);
+    int8_t *const last = NST == 2 ? s1 : NST == 3 ? s2 : s3;
+    for (int k0 = ks;;) {
+        step(s0, last, k0);
+        if ((k0 += BK) >= ke) break;
+        step(s1, s0, k0);
+        if ((k0 += BK) >= ke) break;
+        if (NST > 2) {
+            step(s2, s1, k0);
+            if ((k0 += BK) >= ke) break;
+        }
+        if (NST > 3) {
+            step(s3, s2, k0);
+            if ((k0 += BK) >= ke) break;
+        }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the fills past the end, before the LDS is given back
 
+    if (A.partial) {
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) {
+            const int m = m0 + wm0 + tm * 16 + i16;
+            if (m >= M) continue;
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn) {
+                const int n = n0 + wn0 + tn * 16 + q4 * 4;
+                const int64_t at = ((int64_t)blockIdx.y * A.M + m) * A.N + n;
+                if (P == 1) {
+                    int32_t *o = (int32_t *)A.partial + at;
+                    if (n + 4 <= A.N) __builtin_memcpy(o, &acc[0][tm][tn], 16);
+                    else
+                        for (int r = 0; r < 4; ++r)
+                            if (n + r < A.N) o[r] = acc[0][tm][tn][r];
+                } else {
+                    for (int r = 0; r < 4; ++r)
+                        if (n + r < A.N)
+                            ((int64_t *)A.partial)[at + r] = ((int64_t)acc[0][tm][tn][r] << 16) +
+                                                             ((int64_t)acc[P > 1 ? 1 : 0][tm][tn][r] << 8) +
+                                                             acc[P > 2 ? 2 : 0][tm][tn][r];
+                }
+            }
+        }
+        return;
+    }
+    double sa[TM];
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
         const int m = m0 + wm0 + tm * 16 + i16;
-        if (m >= M) continue;
-        const double sa = A.partial ? 0.0 : (double)A.a_scale[m];
+        sa[tm] = m < M ? (double)A.a_scale[m] : 0.0;
+        if (P == 3) sa[tm] *= 1.0 / (double)I8_FIX;
+    }
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn)
+    for (int tn = 0; tn < TN; ++tn) {
+        const int n = n0 + wn0 + tn * 16 + q4 * 4;
+        double sb[4], bias[4];
+        for (int r = 0; r < 4; ++r) {
+            const int nr = n + r < A.N ? n + r : A.N - 1;
+            sb[r] = A.b_scale ? (double)A.b_scale[nr] : 1.0;
+            bias[r] = A.bias ? (double)A.bias[nr] : 0.0;
+        }
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) {
+            const int m = m0 + wm0 + tm * 16 + i16;
+            float z[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int n = n0 + wn0 + q4 * (4 * TN) + tn * 4 + r;
-                if (n >= A.N) continue;
-                if (A.partial) {
-                    const int64_t at = ((int64_t)blockIdx.y * A.M + m) * A.N + n;
-                    if (P == 1) ((int32_t *)A.partial)[at] = acc[0][tm][tn][r];
-                    else
-                        ((int64_t *)A.partial)[at] = ((int64_t)acc[0][tm][tn][r] << 16) +
-                                                     ((int64_t)acc[P > 1 ? 1 : 0][tm][tn][r] << 8) + acc[P > 2 ? 2 : 0][tm][tn][r];
-                } else {
-                    double s = (double)acc[0][tm][tn][r];
-                    if (P == 3)
-                        s = s * 65536.0 + (double)acc[P > 1 ? 1 : 0][tm][tn][r] * 256.0 + (double)acc[P > 2 ? 2 : 0][tm][tn][r];
-                    li_store1(A, (int64_t)m * A.out_stride + n, li_finish<P>(s, sa, A, n));
-                }
+                double t = (double)acc[0][tm][tn][r];
+                if (P == 3)
+                    t = t * 65536.0 + ((double)acc[P > 1 ? 1 : 0][tm][tn][r] * 256.0 + (double)acc[P > 2 ? 2 : 0][tm][tn][r]);
+                t *= sa[tm];
+                if (P == 1) t = t * sb[r] + bias[r];
+                if (P == 1 && A.relu) t = t < 0.0 ? 0.0 : t; // keeps NaN
+                z[r] = (float)t;
             }
+            if (m >= M || n >= A.N) continue;
+            const int64_t at = (int64_t)m * A.out_stride + n;
+            if (n + 4 <= A.N) li_store4(A, at, z);
+            else
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < A.N) li_store1(A, at + r, z[r]);
+        }
     }
 }
 
 // (The body is a device function: a kernel template with these builtins in it is dropped from the host pass.)
-template <int BM, int BN, int WM, int WN, int P>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64)
+template <int BM, int BN, int WM, int WN, int P, int BK, int NST, int OCC>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, OCC)
 linear_i8_kernel(const LiArgs A)
 {
-    linear_i8_tile<BM, BN, WM, WN, P>(A);
+    linear_i8_tile<BM, BN, WM, WN, P, BK, NST>(A);
 }
 
 // Joins the sums of a split k.
@@ -228,11 +316,27 @@ struct LiPlan {
 };
 
 // Tile by the rows there are; k is split until about every CU has a workgroup, down to 512 bytes each.
+#ifndef LI_C256
+#define LI_C256 256, 256, 128, 64, 1, 64, 4, 2
+#define LI_T256 512
+#endif
+#ifndef LI_C128
+#define LI_C128 128, 128, 64, 64, 1, 64, 4, 2
+#define LI_T128 256
+#endif
+#ifndef LI_C128P
+#define LI_C128P 128, 128, 64, 32, 3, 64, 4, 2
+#define LI_T128P 512
+#endif
+#ifndef LI_BIG
+#define LI_BIG 1
+#endif
 static LiPlan li_plan(int M, int N, int K, int P)
 {
     LiPlan p;
     p.bm = p.bn = 64;
     if (P == 1 && M <= 32) p.bm = 32;
+    else if (LI_BIG && P == 1 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) p.bm = p.bn = 256;
     else if (M > 64 && N > 64) p.bm = p.bn = 128;
     const int64_t tiles = (int64_t)((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
     const int steps = (K + LI_BK - 1) / LI_BK;
@@ -260,13 +364,15 @@ template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *partial,
     const int64_t tiles = (int64_t)A.tiles_m * A.tiles_n;
     FRCNN_REQUIRE(tiles < (1ll << 31), "linear_i8: too many tiles");
     const dim3 grid((unsigned)tiles, p.splits);
-    if (p.bm == 128) {
-        if (P == 1) hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 64, 1>), grid, dim3(256), 0, st, A);
-        else hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 32, 3>), grid, dim3(512), 0, st, A);
+    if (p.bm == 256) {
+        hipLaunchKernelGGL((linear_i8_kernel<LI_C256>), grid, dim3(LI_T256), 0, st, A);
+    } else if (p.bm == 128) {
+        if (P == 1) hipLaunchKernelGGL((linear_i8_kernel<LI_C128>), grid, dim3(LI_T128), 0, st, A);
+        else hipLaunchKernelGGL((linear_i8_kernel<LI_C128P>), grid, dim3(LI_T128P), 0, st, A);
     } else if (p.bm == 64) {
-        hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, P>), grid, dim3(256), 0, st, A);
+        hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, P, 128, 2, 1>), grid, dim3(256), 0, st, A);
     } else {
-        hipLaunchKernelGGL((linear_i8_kernel<32, 64, 16, 32, 1>), grid, dim3(256), 0, st, A);
+        hipLaunchKernelGGL((linear_i8_kernel<32, 64, 16, 32, 1, 128, 2, 1>), grid, dim3(256), 0, st, A);
     }
     FRCNN_CHECK_LAUNCH("linear_i8");
     if (p.splits > 1) {
