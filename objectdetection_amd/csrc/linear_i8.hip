@@ -10,7 +10,8 @@
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-#define LI_BK 128          // bytes of k per LDS stage
+#define LI_BK 64           // bytes of k per LDS stage: one matrix instruction deep
+#define LI_STAGES 4
 #define LI_OOB 0x70000000  // a byte offset beyond every tile: the buffer load returns zeros unread
 #define LI_MAX_STRIDE 4000000 // 256 rows of it stay below LI_OOB
 
@@ -27,42 +28,40 @@ struct LiArgs {
     void *partial;                       // per-split sums, or NULL
 };
 
-// One result from an exact sum.  P = 3: a_scale is the magnitude that the digits are relative to.
-template <int P>
-__device__ __forceinline__ float li_finish(double sum, double a_scale, const LiArgs &A, int n)
+// One result from an exact sum: the scales and the bias in 64 bits, then fp32.
+__device__ __forceinline__ float li_finish(double sum, double a_scale, double b_scale, double bias, int relu)
 {
-    double z = sum * (P == 3 ? a_scale * (1.0 / (double)I8_FIX) : a_scale);
-    if (A.b_scale) z *= (double)A.b_scale[n];
-    if (A.bias) z += (double)A.bias[n];
-    if (A.relu) z = z < 0.0 ? 0.0 : z; // keeps NaN
-    return (float)z;
+    const float z = (float)__builtin_fma(sum * a_scale, b_scale, bias);
+    return relu && z < 0.0f ? 0.0f : z; // keeps NaN
 }
 
-__device__ __forceinline__ void li_store1(const LiArgs &A, int64_t at, float z)
+// sum_p digit_p 2^(8 (2 - p)) of a fixed-point row, or the plain sum
+template <int P> __device__ __forceinline__ double li_sum(int d0, int d1, int d2)
 {
-    if (A.out_type == FRCNN_F32) ((float *)A.out)[at] = z;
-    else if (A.out_type == FRCNN_BF16) ((__bf16 *)A.out)[at] = (__bf16)z;
-    else ((_Float16 *)A.out)[at] = (_Float16)z;
+    const double t = (double)d0;
+    return P == 1 ? t : __builtin_fma(t, 65536.0, __builtin_fma((double)d1, 256.0, (double)d2));
 }
 
-// Four neighbours; the address is aligned to one element.
-__device__ __forceinline__ void li_store4(const LiArgs &A, int64_t at, const float (&z)[4])
+// Four neighbours (the first `count` of them) in out's type; the address is aligned to one element.
+template <typename T> __device__ __forceinline__ void li_store(T *o, const float (&z)[4], int count)
 {
-    if (A.out_type == FRCNN_F32) {
-        __builtin_memcpy((float *)A.out + at, z, 16);
-    } else if (A.out_type == FRCNN_BF16) {
-        const __bf16 h[4] = {(__bf16)z[0], (__bf16)z[1], (__bf16)z[2], (__bf16)z[3]};
-        __builtin_memcpy((__bf16 *)A.out + at, h, 8);
+    T h[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) h[r] = (T)z[r];
+    if (count >= 4) {
+        __builtin_memcpy(o, h, sizeof(h));
     } else {
-        const _Float16 h[4] = {(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]};
-        __builtin_memcpy((_Float16 *)A.out + at, h, 8);
+        if (count > 0) o[0] = h[0];
+        if (count > 1) o[1] = h[1];
+        if (count > 2) o[2] = h[2];
     }
 }
 
-// A stage of LDS holds BK bytes of k for the tile's rows of a (P planes) and of b.  The 16-byte slot of chunk c of row r
-// is c ^ swizzle(r): sixteen consecutive rows, which the lanes of a matrix instruction read together, then cover all 64
-// banks once.
-template <int BK> __device__ __forceinline__ int li_swz(int r) { return BK == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+// A stage of LDS holds LI_BK = 64 bytes of k for the tile's rows of a (P planes) and of b.  The 16-byte slot of chunk c of
+// row r is c ^ swizzle(r).  A 16-byte LDS read serves its lanes in four turns of sixteen, 0-3 with 12-15 and 20-27 first;
+// with the lanes on sixteen rows by four chunks this swizzle puts each turn on all 64 banks once (no conflict counted;
+// (r >> 2) & 3, which spreads lanes 0-15, doubles the cycles).
+__device__ __forceinline__ int li_swz(int r) { return (-(r >> 2)) & 3; }
 
 // Workgroups go to the eight XCDs in turn: neighbours in the tile order go to one XCD, eight tiles of m by all of n, so
 // that its L2 sees a row of a and a row of b several times.
@@ -77,11 +76,12 @@ __device__ __forceinline__ void li_tile(int tiles_m, int tiles_n, int &tm, int &
     tn = rem / gm;
 }
 
-// One tile of BM x BN by waves of WM x WN, k in stages of BK bytes that travel global -> LDS directly, NST stages in
-// flight.
-template <int BM, int BN, int WM, int WN, int P, int BK, int NST>
+// One tile of BM x BN by waves of WM x WN.  k goes by in stages of 64 bytes: global -> LDS directly, LI_STAGES in the
+// ring; LDS -> registers one stage ahead of the matrix instructions; so that a load has LI_STAGES - 1 stages to arrive.
+template <int BM, int BN, int WM, int WN, int P>
 __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
 {
+    constexpr int BK = LI_BK;
     constexpr int NW = (BM / WM) * (BN / WN);
     constexpr int TM = WM / 16, TN = WN / 16;
     constexpr int RPL = 1024 / BK, CPR = BK / 16; // rows a load of 64 x 16 bytes covers, chunks of a row
@@ -91,8 +91,8 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
     static_assert(GA * RPL * NW == BM && GB * RPL * NW == BN, "tile rows have to divide over the waves");
     __shared__ __align__(1024) int8_t s0[STAGE];
     __shared__ __align__(1024) int8_t s1[STAGE];
-    __shared__ __align__(1024) int8_t s2[NST > 2 ? STAGE : 16];
-    __shared__ __align__(1024) int8_t s3[NST > 3 ? STAGE : 16];
+    __shared__ __align__(1024) int8_t s2[STAGE];
+    __shared__ __align__(1024) int8_t s3[STAGE];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -119,38 +119,37 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
 #pragma unroll
     for (int j = 0; j < GA; ++j) {
         const int r = (wave * GA + j) * RPL + lane / CPR;
-        ca[j] = ((lane % CPR) ^ li_swz<BK>(r)) * 16;
+        ca[j] = ((lane % CPR) ^ li_swz(r)) * 16;
         va[j] = r * (int)A.a_stride + ca[j];
     }
 #pragma unroll
     for (int j = 0; j < GB; ++j) {
         const int r = (wave * GB + j) * RPL + lane / CPR;
-        cb[j] = ((lane % CPR) ^ li_swz<BK>(r)) * 16;
+        cb[j] = ((lane % CPR) ^ li_swz(r)) * 16;
         vb[j] = r * (int)A.b_stride + cb[j];
     }
-    // Chunks at and beyond the end of k are not read: their offset is beyond the buffer and the load stores zeros.  A
-    // stage past the end is filled like any other, so that the count of loads in flight is the same in every step.
+    // Load i of a stage.  Chunks at and beyond the end of k are not read: their offset is beyond the buffer and the load
+    // stores zeros.  A stage past the end is filled like any other, so that the loads in flight are the same in every step.
+    auto fill1 = [&](int8_t *s, int k0, int i) {
+        if (i < GA * P) {
+            const int j = i % GA, p = i / GA;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra[p], (lds_void *)(s + (p * BM + (wave * GA + j) * RPL) * BK), 16,
+                                                     k0 + ca[j] < ke ? va[j] : LI_OOB, k0, 0, 0);
+        } else {
+            const int j = i - GA * P;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(s + (P * BM + (wave * GB + j) * RPL) * BK), 16,
+                                                     k0 + cb[j] < ke ? vb[j] : LI_OOB, k0, 0, 0);
+        }
+    };
     auto fill = [&](int8_t *s, int k0) {
 #pragma unroll
-        for (int j = 0; j < GA; ++j) {
-            const int v = k0 + ca[j] < ke ? va[j] : LI_OOB;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra[p], (lds_void *)(s + (p * BM + (wave * GA + j) * RPL) * BK), 16,
-                                                         v, k0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < GB; ++j) {
-            const int v = k0 + cb[j] < ke ? vb[j] : LI_OOB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(s + (P * BM + (wave * GB + j) * RPL) * BK), 16, v, k0, 0,
-                                                     0);
-        }
+        for (int i = 0; i < LPS; ++i) fill1(s, k0, i);
     };
     // the last chunk of k may hold bytes of whatever follows the row: cleared in a's rows
     auto clear_tail = [&](int8_t *s, int k0) {
         for (int r = threadIdx.x; r < P * BM; r += NW * 64) {
             const int c = (A.K - k0) >> 4;
-            int8_t *q = s + r * BK + ((c ^ li_swz<BK>(r % BM)) << 4);
+            int8_t *q = s + r * BK + ((c ^ li_swz(r % BM)) << 4);
             for (int j = A.K & 15; j < 16; ++j) q[j] = 0;
         }
         __syncthreads();
@@ -165,61 +164,65 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn) acc[p][tm][tn] = (i32x4){0, 0, 0, 0};
     // b is the instruction's row operand: a lane's four results are neighbours in n
-    const int swz = li_swz<BK>(i16);
-    auto compute = [&](const int8_t *s) {
-#pragma unroll
-        for (int kk = 0; kk < BK / 64; ++kk) {
-            const int at = i16 * BK + (((kk * 4 + q4) ^ swz) << 4);
-            i32x4 fb[TN];
-#pragma unroll
-            for (int tn = 0; tn < TN; ++tn) fb[tn] = *(const i32x4 *)(s + (P * BM + wn0 + tn * 16) * BK + at);
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-#pragma unroll
-                for (int tm = 0; tm < TM; ++tm) {
-                    const i32x4 fa = *(const i32x4 *)(s + (p * BM + wm0 + tm * 16) * BK + at);
-#pragma unroll
-                    for (int tn = 0; tn < TN; ++tn)
-                        acc[p][tm][tn] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[tn], fa, acc[p][tm][tn], 0, 0, 0);
-                }
-        }
+    const int frag = i16 * BK + ((q4 ^ li_swz(i16)) << 4);
+    struct Frags {
+        i32x4 a[P * TM], b[TN];
     };
-    // One step: this stage's loads are complete in this wave (the NST - 2 later stages may be in flight) and, behind the
-    // barrier, in all; every wave has read the previous stage (lgkmcnt), whose buffer the next fill overwrites.
-    auto step = [&](int8_t *cur, int8_t *next, int k0) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LPS * (NST - 2)) : "memory");
-        fill(next, k0 + (NST - 1) * BK);
-        if (k0 + BK > A.K && (A.K & 15)) clear_tail(cur, k0);
-        compute(cur);
+    Frags f0, f1;
+    auto read1 = [&](Frags &f, const int8_t *s, int i) {
+        if (i < TN) f.b[i] = *(const i32x4 *)(s + (P * BM + wn0 + i * 16) * BK + frag);
+        else f.a[i - TN] = *(const i32x4 *)(s + ((i - TN) / TM * BM + wm0 + (i - TN) % TM * 16) * BK + frag);
+    };
+    // One step multiplies the stage that `f` holds, reads the next one, `next`, into `g`, and refills the buffer `cur` that
+    // `f` came from.  Behind the wait and the barrier the next stage is complete in every wave (the LI_STAGES - 2 later
+    // ones may be in flight) and every wave has read the current one (lgkmcnt).  Reads and loads go out between the matrix
+    // instructions, a few behind each group of TN.
+    auto step = [&](const Frags &f, Frags &g, int8_t *cur, int8_t *next, int k0) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LPS * (LI_STAGES - 2)) : "memory");
+        if (k0 + 2 * BK > A.K && k0 + BK < A.K && (A.K & 15)) clear_tail(next, k0 + BK);
+        constexpr int G = P * TM, R = G > 1 ? (P * TM + TN + G - 2) / (G - 1) : P * TM + TN, L = (LPS + G - 1) / G;
+#pragma unroll
+        for (int t = 0; t < G; ++t) {
+#pragma unroll
+            for (int tn = 0; tn < TN; ++tn)
+                acc[t / TM][t % TM][tn] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.b[tn], f.a[t], acc[t / TM][t % TM][tn], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = t * R; i < (t + 1) * R && i < P * TM + TN; ++i) read1(g, next, i);
+#pragma unroll
+            for (int i = t * L; i < (t + 1) * L && i < LPS; ++i) fill1(cur, k0 + LI_STAGES * BK, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     fill(s0, ks);
-    if (NST > 2) fill(s1, ks + BK);
-    if (NST > 3) fill(s2, ks + 2 * BK);
-    int8_t *const last = NST == 2 ? s1 : NST == 3 ? s2 : s3;
+    fill(s1, ks + BK);
+    fill(s2, ks + 2 * BK);
+    fill(s3, ks + 3 * BK);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LPS * (LI_STAGES - 1)) : "memory");
+    if (ks + BK > A.K && (A.K & 15)) clear_tail(s0, ks);
+#pragma unroll
+    for (int i = 0; i < P * TM + TN; ++i) read1(f0, s0, i);
     for (int k0 = ks;;) {
-        step(s0, last, k0);
+        step(f0, f1, s0, s1, k0);
         if ((k0 += BK) >= ke) break;
-        step(s1, s0, k0);
+        step(f1, f0, s1, s2, k0);
         if ((k0 += BK) >= ke) break;
-        if (NST > 2) {
-            step(s2, s1, k0);
-            if ((k0 += BK) >= ke) break;
-        }
-        if (NST > 3) {
-            step(s3, s2, k0);
-            if ((k0 += BK) >= ke) break;
-        }
+        step(f0, f1, s2, s3, k0);
+        if ((k0 += BK) >= ke) break;
+        step(f1, f0, s3, s0, k0);
+        if ((k0 += BK) >= ke) break;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the fills past the end, before the LDS is given back
 
+    const int mw = m0 + wm0 + i16, nw = n0 + wn0 + q4 * 4;
     if (A.partial) {
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            const int m = m0 + wm0 + tm * 16 + i16;
+            const int m = mw + tm * 16;
             if (m >= M) continue;
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn) {
-                const int n = n0 + wn0 + tn * 16 + q4 * 4;
+                const int n = nw + tn * 16;
                 const int64_t at = ((int64_t)blockIdx.y * A.M + m) * A.N + n;
                 if (P == 1) {
                     int32_t *o = (int32_t *)A.partial + at;
@@ -241,49 +244,43 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
     double sa[TM];
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
-        const int m = m0 + wm0 + tm * 16 + i16;
-        sa[tm] = m < M ? (double)A.a_scale[m] : 0.0;
+        sa[tm] = mw + tm * 16 < M ? (double)A.a_scale[mw + tm * 16] : 0.0;
         if (P == 3) sa[tm] *= 1.0 / (double)I8_FIX;
     }
+    auto write = [&](auto *out) {
 #pragma unroll
-    for (int tn = 0; tn < TN; ++tn) {
-        const int n = n0 + wn0 + tn * 16 + q4 * 4;
-        double sb[4], bias[4];
-        for (int r = 0; r < 4; ++r) {
-            const int nr = n + r < A.N ? n + r : A.N - 1;
-            sb[r] = A.b_scale ? (double)A.b_scale[nr] : 1.0;
-            bias[r] = A.bias ? (double)A.bias[nr] : 0.0;
-        }
-#pragma unroll
-        for (int tm = 0; tm < TM; ++tm) {
-            const int m = m0 + wm0 + tm * 16 + i16;
-            float z[4];
+        for (int tn = 0; tn < TN; ++tn) {
+            const int n = nw + tn * 16;
+            double sb[4], bias[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                double t = (double)acc[0][tm][tn][r];
-                if (P == 3)
-                    t = t * 65536.0 + ((double)acc[P > 1 ? 1 : 0][tm][tn][r] * 256.0 + (double)acc[P > 2 ? 2 : 0][tm][tn][r]);
-                t *= sa[tm];
-                if (P == 1) t = t * sb[r] + bias[r];
-                if (P == 1 && A.relu) t = t < 0.0 ? 0.0 : t; // keeps NaN
-                z[r] = (float)t;
+                const int nr = n + r < A.N ? n + r : A.N - 1;
+                sb[r] = P == 1 ? (double)A.b_scale[nr] : 1.0;
+                bias[r] = P == 1 && A.bias ? (double)A.bias[nr] : 0.0;
             }
-            if (m >= M || n >= A.N) continue;
-            const int64_t at = (int64_t)m * A.out_stride + n;
-            if (n + 4 <= A.N) li_store4(A, at, z);
-            else
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) {
+                const int m = mw + tm * 16;
+                float z[4];
+#pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (n + r < A.N) li_store1(A, at + r, z[r]);
+                    z[r] = li_finish(li_sum<P>(acc[0][tm][tn][r], acc[P > 1 ? 1 : 0][tm][tn][r], acc[P > 2 ? 2 : 0][tm][tn][r]),
+                                     sa[tm], sb[r], bias[r], A.relu);
+                if (m < M) li_store(out + (int64_t)m * A.out_stride + n, z, A.N - n);
+            }
         }
-    }
+    };
+    if (A.out_type == FRCNN_F32) write((float *)A.out);
+    else if (A.out_type == FRCNN_BF16) write((__bf16 *)A.out);
+    else write((_Float16 *)A.out);
 }
 
 // (The body is a device function: a kernel template with these builtins in it is dropped from the host pass.)
-template <int BM, int BN, int WM, int WN, int P, int BK, int NST, int OCC>
+template <int BM, int BN, int WM, int WN, int P, int OCC>
 __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, OCC)
 linear_i8_kernel(const LiArgs A)
 {
-    linear_i8_tile<BM, BN, WM, WN, P, BK, NST>(A);
+    linear_i8_tile<BM, BN, WM, WN, P>(A);
 }
 
 // Joins the sums of a split k.
@@ -306,7 +303,12 @@ linear_i8_join_kernel(const LiArgs A, int splits)
         for (int k = 0; k < splits; ++k) t += ((const int64_t *)A.partial)[k * MN + i];
         s = (double)t;
     }
-    li_store1(A, (int64_t)m * A.out_stride + n, li_finish<P>(s, (double)A.a_scale[m], A, n));
+    const float z = li_finish(s, (double)A.a_scale[m] * (P == 3 ? 1.0 / (double)I8_FIX : 1.0),
+                              P == 1 ? (double)A.b_scale[n] : 1.0, P == 1 && A.bias ? (double)A.bias[n] : 0.0, A.relu);
+    const int64_t at = (int64_t)m * A.out_stride + n;
+    if (A.out_type == FRCNN_F32) ((float *)A.out)[at] = z;
+    else if (A.out_type == FRCNN_BF16) ((__bf16 *)A.out)[at] = (__bf16)z;
+    else ((_Float16 *)A.out)[at] = (_Float16)z;
 }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -316,32 +318,17 @@ struct LiPlan {
 };
 
 // Tile by the rows there are; k is split until about every CU has a workgroup, down to 512 bytes each.
-#ifndef LI_C256
-#define LI_C256 256, 256, 128, 64, 1, 64, 4, 2
-#define LI_T256 512
-#endif
-#ifndef LI_C128
-#define LI_C128 128, 128, 64, 64, 1, 64, 4, 2
-#define LI_T128 256
-#endif
-#ifndef LI_C128P
-#define LI_C128P 128, 128, 64, 32, 3, 64, 4, 2
-#define LI_T128P 512
-#endif
-#ifndef LI_BIG
-#define LI_BIG 1
-#endif
 static LiPlan li_plan(int M, int N, int K, int P)
 {
     LiPlan p;
     p.bm = p.bn = 64;
     if (P == 1 && M <= 32) p.bm = 32;
-    else if (LI_BIG && P == 1 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) p.bm = p.bn = 256;
+    else if (P == 1 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) p.bm = p.bn = 256;
     else if (M > 64 && N > 64) p.bm = p.bn = 128;
     const int64_t tiles = (int64_t)((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
     const int steps = (K + LI_BK - 1) / LI_BK;
     int64_t want = tiles >= 256 ? 1 : 256 / tiles;
-    const int most = steps / 4 > 0 ? steps / 4 : 1;
+    const int most = steps / 8 > 0 ? steps / 8 : 1;
     if (want > most) want = most;
     if (want < 1) want = 1;
     const int per = (steps + (int)want - 1) / (int)want;
@@ -365,14 +352,14 @@ template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *partial,
     FRCNN_REQUIRE(tiles < (1ll << 31), "linear_i8: too many tiles");
     const dim3 grid((unsigned)tiles, p.splits);
     if (p.bm == 256) {
-        hipLaunchKernelGGL((linear_i8_kernel<LI_C256>), grid, dim3(LI_T256), 0, st, A);
+        hipLaunchKernelGGL((linear_i8_kernel<256, 256, 64, 128, 1, 2>), grid, dim3(512), 0, st, A);
     } else if (p.bm == 128) {
-        if (P == 1) hipLaunchKernelGGL((linear_i8_kernel<LI_C128>), grid, dim3(LI_T128), 0, st, A);
-        else hipLaunchKernelGGL((linear_i8_kernel<LI_C128P>), grid, dim3(LI_T128P), 0, st, A);
+        if (P == 1) hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 64, 1, 2>), grid, dim3(256), 0, st, A);
+        else hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 32, 3, 2>), grid, dim3(512), 0, st, A);
     } else if (p.bm == 64) {
-        hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, P, 128, 2, 1>), grid, dim3(256), 0, st, A);
+        hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, P, 1>), grid, dim3(256), 0, st, A);
     } else {
-        hipLaunchKernelGGL((linear_i8_kernel<32, 64, 16, 32, 1, 128, 2, 1>), grid, dim3(256), 0, st, A);
+        hipLaunchKernelGGL((linear_i8_kernel<32, 64, 32, 32, 1, 1>), grid, dim3(128), 0, st, A);
     }
     FRCNN_CHECK_LAUNCH("linear_i8");
     if (p.splits > 1) {
