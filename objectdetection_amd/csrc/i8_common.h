@@ -30,6 +30,72 @@ __device__ __forceinline__ int i8_rows(const int32_t *n_rows, int M)
     return n < 0 ? 0 : (n < M ? n : M);
 }
 
+// ---- the row quantiser's arithmetic ----------------------------------------------------------------------------------
+// top = max_k |x_k|; scale = top / 127 (fp32); code_k = the whole number nearest to the EXACT quotient 127 x_k / top, ties to
+// even: codes do not depend on how a kernel happens to round.  A 32-bit product settles almost every one: t = x * (127 / top)
+// with the hardware's reciprocal (one step off at most) is off by less than 5e-5, so its nearest whole number is right
+// unless t is that close to a half.  There the comparison of 254 |x| with (2 n + 1) top decides, n + 1/2 being the half in
+// question; both products are exact in 64 bits (32 bits each).
+struct QrRow {
+    float top, inv, scale;
+    bool none; // codes are 0
+    bool far;  // the row's numbers have to go through qr_lift first: 1 / top would leave fp32's normal numbers
+    float lift;
+};
+
+__device__ __forceinline__ int qr_code(float x, const QrRow &q)
+{
+    const float t = x * q.inv;
+    const float r = __builtin_rintf(t);
+    if (__builtin_expect(fabsf(t - r) < 0.5f - 1.0e-4f, 1)) return (int)r;
+    const float n = __builtin_floorf(fabsf(t));
+    const double over = 254.0 * fabs((double)x) - (double)(2.0f * n + 1.0f) * (double)q.top;
+    const int c = (int)n + (over > 0.0 || (over == 0.0 && ((int)n & 1)) ? 1 : 0);
+    return x < 0.0f ? -c : c;
+}
+
+__device__ __forceinline__ uint32_t qr_pack(int a, int b, int c, int d)
+{
+    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
+}
+
+// What a row is quantised by, from the largest magnitude's bits (as integers, magnitudes keep their order: Inf above every
+// number, NaN above Inf).  A row with an Inf or a NaN has scale NaN and codes 0: products of it are NaN, never a plausible
+// number.
+__device__ __forceinline__ QrRow qr_row(uint32_t top_bits)
+{
+    QrRow r;
+    const bool finite = top_bits < 0x7f800000u;
+    r.top = __uint_as_float(top_bits);
+    r.none = !finite || top_bits == 0;
+    r.far = r.top < 1e-30f || r.top > 1e30f;
+    r.lift = r.top < 1e-30f ? 1.2676506002282294e30f : 7.888609052210118e-31f; // 2^100, 2^-100
+    // correctly rounded: a quotient of a 24-bit number by 127 keeps 2^-32 away from the middle of two fp32 numbers
+    r.scale = finite ? (float)((double)r.top * (1.0 / 127.0)) : __builtin_nanf("");
+    if (r.far) r.top *= r.lift;
+    r.inv = r.none ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(r.top);
+    return r;
+}
+
+// x by a power of two.  Exact where it counts: what 2^-100 pushes below the normal numbers is below top 2^-120.
+template <typename T> __device__ __forceinline__ T qr_lift(T x, const QrRow &q) { return (T)((float)x * q.lift); }
+
+__device__ __forceinline__ uint32_t qr_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t qr_max(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// Largest value of a workgroup of THREADS; red: THREADS / 64 words of LDS.
+template <int THREADS> __device__ __forceinline__ uint32_t qr_block_max(uint32_t v, uint32_t *red)
+{
+    for (int o = 32; o > 0; o >>= 1) v = qr_max(v, __shfl_xor(v, o));
+    if (THREADS > 64) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) v = qr_max(v, red[w]);
+    }
+    return v;
+}
+
 // A signed 24-bit fixed-point number T (|T| <= I8_FIX) as three signed 8-bit digits, T = d0 2^16 + d1 2^8 + d2 with
 // d0 in [-127, 127] and d1, d2 in [-128, 127].
 #define I8_FIX 8323072 /* 127 * 2^16 */
@@ -45,6 +111,8 @@ __device__ __forceinline__ void i8_digits(int T, int &d0, int &d1, int &d2)
 #define I8_MAX_K 131071
 
 // quantize.hip, used by linear_i8.hip
+int frcnn_i8_quantize(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows, int8_t *codes,
+                      int64_t codes_stride, float *scale, hipStream_t stream);
 int frcnn_i8_pad_rows(const int8_t *src, int64_t src_stride, int rows, int K, int8_t *dst, int64_t dst_stride,
                       hipStream_t stream);
 int frcnn_i8_transpose(const int8_t *src, int64_t src_stride, int rows, int cols, int8_t *dst, int64_t dst_stride,

@@ -25,8 +25,13 @@ struct LiArgs {
     int relu, out_type;
     void *out;
     int64_t out_stride;                  // elements
-    void *partial;                       // per-split sums, or NULL
+    void *partial;                       // sums of a split k, (splits, M, li_ld4(N)) int32 (P = 3: int64), or NULL
+    int splits;
+    int n_group;                         // short rows: output channels of a workgroup
 };
+
+// Row length of a split's sums: quads of neighbours are stored whole
+__host__ __device__ __forceinline__ int li_ld4(int N) { return (N + 3) & ~3; }
 
 // One result from an exact sum: the scales and the bias in 64 bits, then fp32.
 __device__ __forceinline__ float li_finish(double sum, double a_scale, double b_scale, double bias, int relu)
@@ -55,6 +60,13 @@ template <typename T> __device__ __forceinline__ void li_store(T *o, const float
         if (count > 1) o[1] = h[1];
         if (count > 2) o[2] = h[2];
     }
+}
+
+__device__ __forceinline__ void li_store_as(const LiArgs &A, int64_t at, float z)
+{
+    if (A.out_type == FRCNN_F32) ((float *)A.out)[at] = z;
+    else if (A.out_type == FRCNN_BF16) ((__bf16 *)A.out)[at] = (__bf16)z;
+    else ((_Float16 *)A.out)[at] = (_Float16)z;
 }
 
 // A stage of LDS holds LI_BK = 64 bytes of k for the tile's rows of a (P planes) and of b.  The 16-byte slot of chunk c of
@@ -215,7 +227,7 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the fills past the end, before the LDS is given back
 
     const int mw = m0 + wm0 + i16, nw = n0 + wn0 + q4 * 4;
-    if (A.partial) {
+    if (A.splits > 1) {
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
             const int m = mw + tm * 16;
@@ -223,19 +235,17 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn) {
                 const int n = nw + tn * 16;
-                const int64_t at = ((int64_t)blockIdx.y * A.M + m) * A.N + n;
+                if (n >= A.N) continue;
+                const int64_t at = ((int64_t)blockIdx.y * A.M + m) * li_ld4(A.N) + n;
                 if (P == 1) {
-                    int32_t *o = (int32_t *)A.partial + at;
-                    if (n + 4 <= A.N) __builtin_memcpy(o, &acc[0][tm][tn], 16);
-                    else
-                        for (int r = 0; r < 4; ++r)
-                            if (n + r < A.N) o[r] = acc[0][tm][tn][r];
+                    *(i32x4 *)((int32_t *)A.partial + at) = acc[0][tm][tn];
                 } else {
+                    int64_t v[4];
+#pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (n + r < A.N)
-                            ((int64_t *)A.partial)[at + r] = ((int64_t)acc[0][tm][tn][r] << 16) +
-                                                             ((int64_t)acc[P > 1 ? 1 : 0][tm][tn][r] << 8) +
-                                                             acc[P > 2 ? 2 : 0][tm][tn][r];
+                        v[r] = ((int64_t)acc[0][tm][tn][r] << 16) + ((int64_t)acc[P > 1 ? 1 : 0][tm][tn][r] << 8) +
+                               acc[P > 2 ? 2 : 0][tm][tn][r];
+                    __builtin_memcpy(__builtin_assume_aligned((int64_t *)A.partial + at, 16), v, 32);
                 }
             }
         }
@@ -282,42 +292,332 @@ linear_i8_kernel(const LiArgs A)
 {
     linear_i8_tile<BM, BN, WM, WN, P>(A);
 }
-
-// Joins the sums of a split k.
+// Joins the sums of a split k: a lane takes four neighbours.  (Letting the split that arrives last do this, behind a
+// device-scope fence, was tried: the fence writes back the whole L2 and the product of 2,000 x 12,544 x 1,024 went from 44
+// to 165 us.)
 template <int P>
-__global__ void __launch_bounds__(256)
-linear_i8_join_kernel(const LiArgs A, int splits)
+__global__ void __launch_bounds__(64)
+linear_i8_join_kernel(const LiArgs A)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t MN = (int64_t)A.M * A.N;
-    if (i >= MN) return;
-    const int m = (int)(i / A.N), n = (int)(i - (int64_t)m * A.N);
+    const int quads = li_ld4(A.N) / 4;
+    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
     if (m >= i8_rows(A.n_rows, A.M)) return;
-    double s;
-    if (P == 1) {
-        int32_t t = 0;
-        for (int k = 0; k < splits; ++k) t += ((const int32_t *)A.partial)[k * MN + i];
-        s = (double)t;
-    } else {
-        int64_t t = 0;
-        for (int k = 0; k < splits; ++k) t += ((const int64_t *)A.partial)[k * MN + i];
-        s = (double)t;
+    const int64_t step = (int64_t)A.M * quads;
+    int64_t t[4] = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int k = 0; k < A.splits; ++k) {
+        if (P == 1) {
+            const i32x4 v = ((const i32x4 *)A.partial)[k * step + i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] += v[r];
+        } else {
+            int64_t v[4];
+            __builtin_memcpy(v, __builtin_assume_aligned((const int64_t *)A.partial + (k * step + i) * 4, 16), 32);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] += v[r];
+        }
     }
-    const float z = li_finish(s, (double)A.a_scale[m] * (P == 3 ? 1.0 / (double)I8_FIX : 1.0),
-                              P == 1 ? (double)A.b_scale[n] : 1.0, P == 1 && A.bias ? (double)A.bias[n] : 0.0, A.relu);
+    const double a_scale = (double)A.a_scale[m] * (P == 3 ? 1.0 / (double)I8_FIX : 1.0);
+    float z[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int nr = n + r < A.N ? n + r : A.N - 1;
+        z[r] = li_finish((double)t[r], a_scale, P == 1 ? (double)A.b_scale[nr] : 1.0,
+                         P == 1 && A.bias ? (double)A.bias[nr] : 0.0, A.relu);
+    }
     const int64_t at = (int64_t)m * A.out_stride + n;
-    if (A.out_type == FRCNN_F32) ((float *)A.out)[at] = z;
-    else if (A.out_type == FRCNN_BF16) ((__bf16 *)A.out)[at] = (__bf16)z;
-    else ((_Float16 *)A.out)[at] = (_Float16)z;
+    if (A.out_type == FRCNN_F32) li_store((float *)A.out + at, z, A.N - n);
+    else if (A.out_type == FRCNN_BF16) li_store((__bf16 *)A.out + at, z, A.N - n);
+    else li_store((_Float16 *)A.out + at, z, A.N - n);
+}
+
+// ---- a few rows -----------------------------------------------------------------------------------------------------
+// One launch from float rows (or codes) to the result: a workgroup takes LF_N output channels and all of k.  A thread owns
+// the 16-byte chunks t, t + 1024, ... of k, of the weight rows and of x alike, so that it needs nothing of its neighbours but
+// the row's maximum and the final sum; the weights, which are all there is to read, stay in its registers for every row of
+// x.  Each workgroup quantises x for itself, out of the L2.
+#define LF_THREADS 1024
+#define LF_N 4
+#define LF_CHUNKS 2 // of a thread: k up to 32,768
+
+template <typename T>
+__global__ void __launch_bounds__(LF_THREADS)
+linear_i8_few_kernel(const T *__restrict__ x, int64_t x_stride, const float *__restrict__ x_scale, const LiArgs A)
+{
+    __shared__ uint32_t red[LF_THREADS / 64];
+    __shared__ int sums[LF_THREADS / 64][LF_N];
+    const int n0 = blockIdx.x * LF_N, t = threadIdx.x, K = A.K;
+    const int kf = K & ~15, tail = kf + t < K && t < 16; // the last K % 16 elements: one a lane of the first wave
+    i32x4 w[LF_N][LF_CHUNKS];
+    int w_tail[LF_N];
+#pragma unroll
+    for (int r = 0; r < LF_N; ++r) {
+        const int8_t *b = A.b + (int64_t)(n0 + r < A.N ? n0 + r : A.N - 1) * A.b_stride;
+#pragma unroll
+        for (int i = 0; i < LF_CHUNKS; ++i) {
+            const int k = (i * LF_THREADS + t) * 16;
+            w[r][i] = (i32x4){0, 0, 0, 0};
+            if (k < kf) __builtin_memcpy(&w[r][i], b + k, 16);
+        }
+        w_tail[r] = tail ? b[kf + t] : 0;
+    }
+    const int M = i8_rows(A.n_rows, A.M);
+#pragma unroll 1
+    for (int m = 0; m < M; ++m) {
+        i32x4 q[LF_CHUNKS];
+        int q_tail = 0;
+        float scale;
+        const T *xr = x + m * x_stride;
+        if constexpr (sizeof(T) == 1) {
+#pragma unroll
+            for (int i = 0; i < LF_CHUNKS; ++i) {
+                const int k = (i * LF_THREADS + t) * 16;
+                q[i] = (i32x4){0, 0, 0, 0};
+                if (k < kf) __builtin_memcpy(&q[i], xr + k, 16);
+            }
+            if (tail) q_tail = xr[kf + t];
+            scale = x_scale[m];
+        } else {
+            I8Vec<T, 16> v[LF_CHUNKS];
+            uint32_t top_bits = 0;
+            float v_tail = tail ? (float)xr[kf + t] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < LF_CHUNKS; ++i) {
+                const int k = (i * LF_THREADS + t) * 16;
+                if (k < kf) v[i] = i8_load<T, 16>(xr + k);
+            }
+            top_bits = qr_bits(v_tail);
+#pragma unroll
+            for (int i = 0; i < LF_CHUNKS; ++i)
+                if ((i * LF_THREADS + t) * 16 < kf)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) top_bits = qr_max(top_bits, qr_bits((float)v[i].v[j]));
+            const QrRow row = qr_row(qr_block_max<LF_THREADS>(top_bits, red));
+            scale = row.scale;
+            if (__builtin_expect(row.far, 0)) {
+                v_tail = qr_lift(v_tail, row);
+#pragma unroll
+                for (int i = 0; i < LF_CHUNKS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[i].v[j] = qr_lift(v[i].v[j], row);
+            }
+            if (!row.none) q_tail = qr_code(v_tail, row);
+#pragma unroll
+            for (int i = 0; i < LF_CHUNKS; ++i) {
+                q[i] = (i32x4){0, 0, 0, 0};
+                if ((i * LF_THREADS + t) * 16 < kf && !row.none)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        q[i][j] = (int)qr_pack(qr_code((float)v[i].v[4 * j], row), qr_code((float)v[i].v[4 * j + 1], row),
+                                               qr_code((float)v[i].v[4 * j + 2], row), qr_code((float)v[i].v[4 * j + 3], row));
+            }
+        }
+        int sum[LF_N];
+#pragma unroll
+        for (int r = 0; r < LF_N; ++r) {
+            sum[r] = q_tail * w_tail[r];
+#pragma unroll
+            for (int i = 0; i < LF_CHUNKS; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[r] = __builtin_amdgcn_sdot4(q[i][j], w[r][i][j], sum[r], false);
+            for (int o = 32; o > 0; o >>= 1) sum[r] += __shfl_xor(sum[r], o);
+        }
+        if ((t & 63) == 0)
+#pragma unroll
+            for (int r = 0; r < LF_N; ++r) sums[t >> 6][r] = sum[r];
+        __syncthreads();
+        if (t < LF_N && n0 + t < A.N) {
+            int total = 0;
+            for (int v = 0; v < LF_THREADS / 64; ++v) total += sums[v][t];
+            const int n = n0 + t;
+            const float z = li_finish((double)total, (double)scale, (double)A.b_scale[n], A.bias ? (double)A.bias[n] : 0.0, A.relu);
+            li_store_as(A, m * A.out_stride + n, z);
+        }
+        __syncthreads(); // red and sums are the next row's
+    }
+}
+
+// ---- short rows ------------------------------------------------------------------------------------------------------
+// For k up to LR_K the codes of BM rows stay in LDS: one launch, x read once, no codes in memory.  First each wave quantises
+// its BM / 8 rows, up to four at a time so that their chains of dependent operations overlap; then it multiplies all BM rows
+// with 16 output channels of its own, whose weights it takes straight from the L2 into registers (no two waves of a workgroup
+// want the same ones), LR_AHEAD steps ahead.  blockIdx.y: a group of output channels; with few rows the groups are what
+// fills the chip, and each quantises for itself.
+#define LR_THREADS 512
+#define LR_K 1024
+#define LR_AHEAD 8
+
+// 16-byte slot of chunk c in row r: rows lie a multiple of 256 bytes apart, the sixteen rows a matrix instruction reads
+// differ in the slot instead
+__device__ __forceinline__ int lr_slot(int c, int r) { return (c & ~15) | ((c ^ r) & 15); }
+
+template <typename T, int BM>
+__device__ __forceinline__ void linear_i8_short(const T *__restrict__ x, int64_t x_stride, const LiArgs &A)
+{
+    constexpr int NW = LR_THREADS / 64, TM = BM / 16, V = 16 / sizeof(T), D = LR_AHEAD;
+    constexpr int ROWS = BM / NW < 4 ? BM / NW : 4;
+    constexpr int NV = LR_K / (64 * V); // loads of a lane per row
+    extern __shared__ __align__(1024) int8_t codes[]; // BM rows of kp bytes
+    __shared__ float scales[BM];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int M = i8_rows(A.n_rows, A.M), K = A.K;
+    const int m0 = blockIdx.x * BM;
+    if (m0 >= M) return;
+    const int rows = M - m0 < BM ? M - m0 : BM;
+    const int kp = (K + 255) & ~255, steps = (K + 63) >> 6;
+    const int kf = K - K % V, tail = kf + lane < K && lane < V; // whole vectors up to kf; the last K % V elements one a lane
+    // rows wave, wave + NW, ...; a row behind the last is the last again: nothing of it is stored
+#pragma unroll 1
+    for (int batch = 0; batch < BM / (NW * ROWS) && batch * ROWS * NW + wave < rows; ++batch) {
+        I8Vec<T, V> v[ROWS][NV];
+        T v_tail[ROWS];
+        uint32_t top_bits[ROWS];
+#pragma unroll
+        for (int g = 0; g < ROWS; ++g) {
+            const int r = (batch * ROWS + g) * NW + wave;
+            const T *xr = x + (int64_t)(m0 + (r < rows ? r : rows - 1)) * x_stride;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int k = (i * 64 + lane) * V;
+                v[g][i] = I8Vec<T, V>{};
+                if (k < kf) v[g][i] = i8_load<T, V>(xr + k);
+            }
+            v_tail[g] = tail ? xr[kf + lane] : (T)0.0f;
+        }
+#pragma unroll
+        for (int g = 0; g < ROWS; ++g) {
+            top_bits[g] = qr_bits((float)v_tail[g]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) top_bits[g] = qr_max(top_bits[g], qr_bits((float)v[g][i].v[j]));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+            for (int g = 0; g < ROWS; ++g) top_bits[g] = qr_max(top_bits[g], __shfl_xor(top_bits[g], o));
+#pragma unroll
+        for (int g = 0; g < ROWS; ++g) {
+            const int r = (batch * ROWS + g) * NW + wave;
+            const QrRow q = qr_row(top_bits[g]);
+            if (lane == 0) scales[r] = q.scale;
+            if (__builtin_expect(q.far, 0)) {
+                v_tail[g] = qr_lift(v_tail[g], q);
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[g][i].v[j] = qr_lift(v[g][i].v[j], q);
+            }
+            int8_t *row = codes + r * kp;
+            if (kf < steps * 64) { // zeros in the last step's 64 bytes, and codes over them
+                const int k = (kf & ~63) + lane;
+                row[lr_slot(k >> 4, r) * 16 + (k & 15)] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int k = (i * 64 + lane) * V;
+                if (k < kf) {
+                    uint32_t p[V / 4];
+#pragma unroll
+                    for (int j = 0; j < V / 4; ++j) {
+                        int c[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[e] = q.none ? 0 : qr_code((float)v[g][i].v[4 * j + e], q);
+                        p[j] = qr_pack(c[0], c[1], c[2], c[3]);
+                    }
+                    __builtin_memcpy(__builtin_assume_aligned(row + lr_slot(k >> 4, r) * 16 + (k & 15), V), p, V);
+                }
+            }
+            if (tail)
+                row[lr_slot((kf + lane) >> 4, r) * 16 + ((kf + lane) & 15)] = (int8_t)(q.none ? 0 : qr_code((float)v_tail[g], q));
+        }
+    }
+    __syncthreads();
+    const int i16 = lane & 15, q4 = lane >> 4;
+    const int n_end = A.n_group * (blockIdx.y + 1) < A.N ? A.n_group * (blockIdx.y + 1) : A.N;
+    const int full = K >> 6; // steps of 64 whole; K & 63: one more, cut
+    double sa[TM];
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) sa[tm] = (double)scales[tm * 16 + i16];
+    for (int n0 = A.n_group * blockIdx.y + wave * 16; n0 < n_end; n0 += NW * 16) {
+        i32x4 fb[D], fl, acc[TM];
+        const int8_t *b = A.b + (int64_t)(n0 + i16 < A.N ? n0 + i16 : A.N - 1) * A.b_stride + q4 * 16;
+#pragma unroll
+        for (int tm = 0; tm < TM; ++tm) acc[tm] = (i32x4){0, 0, 0, 0};
+        auto multiply = [&](const i32x4 &f, int step) {
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) {
+                const int r = tm * 16 + i16;
+                const i32x4 fa = *(const i32x4 *)(codes + r * kp + lr_slot(step * 4 + q4, r) * 16);
+                acc[tm] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, fa, acc[tm], 0, 0, 0);
+            }
+        };
+        // The step that K ends in: a's codes are zeros behind K, so only what lies behind the last weight must not be
+        // read: such an address is moved back, and the bytes are shifted to where they belong.
+        if (K & 63) {
+            const int8_t *end = A.b + (int64_t)(A.N - 1) * A.b_stride + K - 16, *p = b + full * 64;
+            const int over = p > end ? (int)(p - end) : 0;
+            uint64_t h[2];
+            __builtin_memcpy(h, p - over, 16);
+            const int bits = (over & 7) * 8;
+            uint64_t lo = over & 8 ? h[1] : h[0], hi = over & 8 ? 0 : h[1];
+            lo = bits ? lo >> bits | hi << (64 - bits) : lo;
+            hi >>= bits;
+            if (over >= 16) lo = hi = 0;
+            fl = (i32x4){(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (d < full) __builtin_memcpy(&fb[d], b + d * 64, 16);
+        for (int s = 0; s < full; s += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                if (s + d < full) multiply(fb[d], s + d);
+                if (s + d + D < full) __builtin_memcpy(&fb[d], b + (s + d + D) * 64, 16);
+            }
+        }
+        if (K & 63) multiply(fl, full);
+        auto write = [&](auto *out) {
+            const int n = n0 + q4 * 4;
+            double sb[4], bias[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int nr = n + r < A.N ? n + r : A.N - 1;
+                sb[r] = (double)A.b_scale[nr];
+                bias[r] = A.bias ? (double)A.bias[nr] : 0.0;
+            }
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm) {
+                const int m = m0 + tm * 16 + i16;
+                float z[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[r] = li_finish((double)acc[tm][r], sa[tm], sb[r], bias[r], A.relu);
+                if (m < M) li_store(out + (int64_t)m * A.out_stride + n, z, n_end - n);
+            }
+        };
+        if (A.out_type == FRCNN_F32) write((float *)A.out);
+        else if (A.out_type == FRCNN_BF16) write((__bf16 *)A.out);
+        else write((_Float16 *)A.out);
+    }
+}
+
+template <typename T, int BM>
+__global__ void __launch_bounds__(LR_THREADS, 4)
+linear_i8_short_kernel(const T *__restrict__ x, int64_t x_stride, const LiArgs A)
+{
+    linear_i8_short<T, BM>(x, x_stride, A);
 }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct LiPlan {
     int bm, bn, splits, k_split;
+    int64_t tiles;
 };
 
-// Tile by the rows there are; k is split until about every CU has a workgroup, down to 512 bytes each.
+// Tile by the rows there are; k is split until about every CU has a workgroup, down to eight stages each.
 static LiPlan li_plan(int M, int N, int K, int P)
 {
     LiPlan p;
@@ -325,9 +625,9 @@ static LiPlan li_plan(int M, int N, int K, int P)
     if (P == 1 && M <= 32) p.bm = 32;
     else if (P == 1 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) p.bm = p.bn = 256;
     else if (M > 64 && N > 64) p.bm = p.bn = 128;
-    const int64_t tiles = (int64_t)((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
+    p.tiles = (int64_t)((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
     const int steps = (K + LI_BK - 1) / LI_BK;
-    int64_t want = tiles >= 256 ? 1 : 256 / tiles;
+    int64_t want = p.tiles >= 256 ? 1 : 256 / p.tiles;
     const int most = steps / 8 > 0 ? steps / 8 : 1;
     if (want > most) want = most;
     if (want < 1) want = 1;
@@ -337,20 +637,20 @@ static LiPlan li_plan(int M, int N, int K, int P)
     return p;
 }
 
-static size_t li_partial_bytes(const LiPlan &p, int M, int N, int P)
+static size_t li_split_bytes(const LiPlan &p, int M, int N, int P)
 {
-    return p.splits > 1 ? up256((size_t)p.splits * M * N * (P == 3 ? 8 : 4)) : 0;
+    return p.splits > 1 ? (size_t)p.splits * M * li_ld4(N) * (P == 3 ? 8 : 4) : 0;
 }
 
-template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *partial, hipStream_t st)
+template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *split, hipStream_t st)
 {
     A.tiles_m = (A.M + p.bm - 1) / p.bm;
     A.tiles_n = (A.N + p.bn - 1) / p.bn;
     A.k_split = p.k_split;
-    A.partial = p.splits > 1 ? partial : nullptr;
-    const int64_t tiles = (int64_t)A.tiles_m * A.tiles_n;
-    FRCNN_REQUIRE(tiles < (1ll << 31), "linear_i8: too many tiles");
-    const dim3 grid((unsigned)tiles, p.splits);
+    A.splits = p.splits;
+    A.partial = split;
+    FRCNN_REQUIRE(p.tiles < (1ll << 31), "linear_i8: too many tiles");
+    const dim3 grid((unsigned)p.tiles, p.splits);
     if (p.bm == 256) {
         hipLaunchKernelGGL((linear_i8_kernel<256, 256, 64, 128, 1, 2>), grid, dim3(512), 0, st, A);
     } else if (p.bm == 128) {
@@ -363,8 +663,8 @@ template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *partial,
     }
     FRCNN_CHECK_LAUNCH("linear_i8");
     if (p.splits > 1) {
-        const int64_t MN = (int64_t)A.M * A.N;
-        hipLaunchKernelGGL((linear_i8_join_kernel<P>), dim3((unsigned)((MN + 255) / 256)), dim3(256), 0, st, A, p.splits);
+        const int64_t quads = (int64_t)A.M * (li_ld4(A.N) / 4);
+        hipLaunchKernelGGL((linear_i8_join_kernel<P>), dim3((unsigned)((quads + 63) / 64)), dim3(64), 0, st, A);
         FRCNN_CHECK_LAUNCH("linear_i8_join");
     }
     return FRCNN_OK;
@@ -382,11 +682,86 @@ static bool li_in_place(const void *p, int64_t stride, int K)
 
 static bool li_shape_ok(int M, int N, int K) { return M >= 0 && N > 0 && K > 0 && K <= I8_MAX_K && (int64_t)M * N < (1ll << 40); }
 
+// The few-rows form.  1,024 channels, rows of 12,544: 1 / 2 / 3 / 4 rows 5.5 / 8.6 / 11.9 / 15.2 us against 14.5 by tiles and
+// three launches, which cost the host 6 us more than one.
+static bool lf_takes(int M, int K) { return M <= 4 && K <= LF_THREADS * LF_CHUNKS * 16; }
+
+// The short-rows form (K >= 16: the last weight is read by a 16-byte load).  It reads the weights once per BM rows, so it
+// gives way to quantiser and tiles where rows and channels are both many: rows of 1,024, us against us, at 105 channels
+// 8.9 : 11.2 (500 rows), 9.2 : 13.8 (2,000), 36 : 42 (32,000); at 256 9.6 : 12.3, 10.6 : 16.5, 45 : 48; at 1,024 10.4 : 15.0,
+// 20.2 : 24.5, 102 : 97 (and 4,000 rows 31 : 23).
+static bool lr_takes(int M, int N, int K)
+{
+    return K <= LR_K && K >= 16 && M > 2 && (N <= 256 || (int64_t)M * N <= (1 << 21));
+}
+
+template <typename T>
+static int lf_launch(const LiArgs &A, const T *x, int64_t x_stride, const float *x_scale, hipStream_t st)
+{
+    hipLaunchKernelGGL((linear_i8_few_kernel<T>), dim3((A.N + LF_N - 1) / LF_N), dim3(LF_THREADS), 0, st, x, x_stride, x_scale, A);
+    FRCNN_CHECK_LAUNCH("linear_i8_few");
+    return FRCNN_OK;
+}
+
+template <typename T, int BM> static int lr_launch(LiArgs A, const T *x, int64_t x_stride, hipStream_t st)
+{
+    const int tiles = (A.M + BM - 1) / BM;
+    int groups = tiles >= 256 ? 1 : 256 / tiles;
+    const int most = (A.N + LR_THREADS / 4 - 1) / (LR_THREADS / 4); // 16 channels a wave
+    if (groups > most) groups = most;
+    A.n_group = ((A.N + groups - 1) / groups + 3) & ~3;
+    const size_t lds = (size_t)BM * ((A.K + 255) & ~255);
+    static size_t granted[FRCNN_MAX_DEVICES];
+    if (frcnn_reserve_dynamic_lds((const void *)linear_i8_short_kernel<T, BM>, lds, granted) != hipSuccess) {
+        frcnn_set_error("linear_i8_short: %zu bytes of LDS refused", lds);
+        return FRCNN_ELAUNCH;
+    }
+    hipLaunchKernelGGL((linear_i8_short_kernel<T, BM>), dim3(tiles, (A.N + A.n_group - 1) / A.n_group), dim3(LR_THREADS), lds,
+                       st, x, x_stride, A);
+    FRCNN_CHECK_LAUNCH("linear_i8_short");
+    return FRCNN_OK;
+}
+
+// 64 rows a workgroup where those fill the chip, 16 where they do not
+template <typename T> static int lr_run(const LiArgs &A, const T *x, int64_t x_stride, hipStream_t st)
+{
+    const int64_t full = (int64_t)((A.M + 63) / 64) * ((A.N + LR_THREADS / 4 - 1) / (LR_THREADS / 4));
+    return full >= 256 ? lr_launch<T, 64>(A, x, x_stride, st) : lr_launch<T, 16>(A, x, x_stride, st);
+}
+
+// A row of codes brought to an aligned stride where it is not read in place; *p and *stride become what is read.
+static int li_in_rows(const int8_t **p, int64_t *stride, int rows, int K, char *copy, hipStream_t st)
+{
+    const int64_t ld = li_stride(K);
+    if (rows == 1) *stride = ld;
+    if (li_in_place(*p, *stride, K)) return FRCNN_OK;
+    const int rc = frcnn_i8_pad_rows(*p, *stride, rows, K, (int8_t *)copy, ld, st);
+    *p = (const int8_t *)copy;
+    *stride = ld;
+    return rc;
+}
+
+static LiArgs li_args(const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b, int64_t b_stride,
+                      const float *b_scale, const float *bias, int relu, int M, int N, int K, const int32_t *n_rows, void *out,
+                      int out_type, int64_t out_stride)
+{
+    LiArgs A = {};
+    A.a = a; A.a_stride = a_stride; A.a_scale = a_scale;
+    A.b = b; A.b_stride = b_stride; A.b_scale = b_scale;
+    A.bias = bias; A.relu = relu;
+    A.M = M; A.N = N; A.K = K; A.n_rows = n_rows;
+    A.out = out; A.out_type = out_type; A.out_stride = out_stride;
+    return A;
+}
+
+// Workspace: [sums of a split k][codes of b on an aligned stride][codes of a on an aligned stride][a's scales]
+static size_t li_ws_b(int M, int N, int K) { return up256(li_split_bytes(li_plan(M, N, K, 1), M, N, 1)); }
+static size_t li_ws_a(int M, int N, int K) { return li_ws_b(M, N, K) + up256((size_t)N * li_stride(K)); }
+static size_t li_ws_scale(int M, int N, int K) { return li_ws_a(M, N, K) + up256((size_t)M * li_stride(K)); }
+
 extern "C" size_t frcnn_matmul_i8_workspace_bytes(int M, int N, int K)
 {
-    if (!li_shape_ok(M, N, K) || M == 0) return 0;
-    // rows of a and b copied to an aligned stride where the caller's are not, and the sums of a split k
-    return up256((size_t)M * li_stride(K)) + up256((size_t)N * li_stride(K)) + li_partial_bytes(li_plan(M, N, K, 1), M, N, 1);
+    return !li_shape_ok(M, N, K) || M == 0 || lf_takes(M, K) ? 0 : li_ws_scale(M, N, K);
 }
 
 extern "C" int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a_scale, const int8_t *b, int64_t b_stride,
@@ -400,48 +775,23 @@ extern "C" int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a
     if (M == 0) return FRCNN_OK;
     FRCNN_REQUIRE(a && a_scale && b && b_scale && out, "matmul_i8: null pointer");
     hipStream_t st = (hipStream_t)stream;
-    const LiPlan p = li_plan(M, N, K, 1);
-    char *ws = (char *)workspace;
-    const size_t need = frcnn_matmul_i8_workspace_bytes(M, N, K);
-    if (workspace_bytes < need || (need && !workspace)) {
+    LiArgs A = li_args(a, a_stride, a_scale, b, b_stride, b_scale, bias, relu, M, N, K, n_rows, out, out_type, out_stride);
+    if (lf_takes(M, K)) return lf_launch(A, a, a_stride, a_scale, st);
+    const size_t need = li_ws_scale(M, N, K);
+    if (workspace_bytes < need || !workspace) {
         frcnn_set_error("matmul_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
         return FRCNN_EWORKSPACE;
     }
-    const int64_t ld = li_stride(K);
-    LiArgs A = {};
-    if (M == 1) a_stride = ld;
-    if (li_in_place(a, a_stride, K)) {
-        A.a = a;
-        A.a_stride = a_stride;
-    } else {
-        int rc = frcnn_i8_pad_rows(a, a_stride, M, K, (int8_t *)ws, ld, st);
-        if (rc != FRCNN_OK) return rc;
-        A.a = (const int8_t *)ws;
-        A.a_stride = ld;
-    }
-    ws += up256((size_t)M * ld);
-    if (N == 1) b_stride = ld;
-    if (li_in_place(b, b_stride, K)) {
-        A.b = b;
-        A.b_stride = b_stride;
-    } else {
-        int rc = frcnn_i8_pad_rows(b, b_stride, N, K, (int8_t *)ws, ld, st);
-        if (rc != FRCNN_OK) return rc;
-        A.b = (const int8_t *)ws;
-        A.b_stride = ld;
-    }
-    ws += up256((size_t)N * ld);
-    A.n_rows = n_rows;
-    A.M = M; A.N = N; A.K = K;
-    A.a_scale = a_scale; A.b_scale = b_scale; A.bias = bias;
-    A.relu = relu; A.out_type = out_type; A.out = out; A.out_stride = out_stride;
-    return li_launch<1>(A, p, ws, st);
+    const LiPlan p = li_plan(M, N, K, 1);
+    char *ws = (char *)workspace;
+    int rc = li_in_rows(&A.a, &A.a_stride, M, K, ws + li_ws_a(M, N, K), st);
+    if (rc == FRCNN_OK) rc = li_in_rows(&A.b, &A.b_stride, N, K, ws + li_ws_b(M, N, K), st);
+    return rc == FRCNN_OK ? li_launch<1>(A, p, ws, st) : rc;
 }
 
 extern "C" size_t frcnn_linear_i8_workspace_bytes(int M, int N, int K)
 {
-    if (!li_shape_ok(M, N, K) || M == 0) return 0;
-    return up256((size_t)M * 4) + up256((size_t)M * li_stride(K)) + frcnn_matmul_i8_workspace_bytes(M, N, K);
+    return !li_shape_ok(M, N, K) || M == 0 || lf_takes(M, K) || lr_takes(M, N, K) ? 0 : li_ws_scale(M, N, K) + up256((size_t)M * 4);
 }
 
 extern "C" int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, const int8_t *b, int64_t b_stride,
@@ -450,26 +800,43 @@ extern "C" int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, cons
                                size_t workspace_bytes, void *stream)
 {
     FRCNN_REQUIRE(li_shape_ok(M, N, K), "linear_i8: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(i8_type_ok(x_type) && i8_type_ok(out_type), "linear_i8: unknown element type");
+    FRCNN_REQUIRE(x_stride >= 0 && b_stride >= 0 && out_stride >= N, "linear_i8: bad strides");
     if (M == 0) return FRCNN_OK;
+    FRCNN_REQUIRE(x && b && b_scale && out, "linear_i8: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    LiArgs A = li_args(nullptr, li_stride(K), nullptr, b, b_stride, b_scale, bias, relu, M, N, K, n_rows, out, out_type,
+                       out_stride);
+    if (lr_takes(M, N, K)) {
+        if (x_type == FRCNN_F32) return lr_run(A, (const float *)x, x_stride, st);
+        if (x_type == FRCNN_BF16) return lr_run(A, (const __bf16 *)x, x_stride, st);
+        return lr_run(A, (const _Float16 *)x, x_stride, st);
+    }
+    if (lf_takes(M, K)) {
+        if (x_type == FRCNN_F32) return lf_launch(A, (const float *)x, x_stride, nullptr, st);
+        if (x_type == FRCNN_BF16) return lf_launch(A, (const __bf16 *)x, x_stride, nullptr, st);
+        return lf_launch(A, (const _Float16 *)x, x_stride, nullptr, st);
+    }
     const size_t need = frcnn_linear_i8_workspace_bytes(M, N, K);
     if (workspace_bytes < need || !workspace) {
         frcnn_set_error("linear_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
         return FRCNN_EWORKSPACE;
     }
+    const LiPlan p = li_plan(M, N, K, 1);
     char *ws = (char *)workspace;
-    float *a_scale = (float *)ws;
-    int8_t *a = (int8_t *)(ws + up256((size_t)M * 4));
-    char *rest = (char *)a + up256((size_t)M * li_stride(K));
-    int rc = frcnn_quantize_rows_i8(x, x_type, x_stride, M, K, n_rows, a, li_stride(K), a_scale, stream);
-    if (rc != FRCNN_OK) return rc;
-    return frcnn_matmul_i8(a, li_stride(K), a_scale, b, b_stride, b_scale, bias, relu, M, N, K, n_rows, out, out_type,
-                           out_stride, rest, workspace_bytes - (size_t)(rest - ws), stream);
+    int8_t *codes = (int8_t *)(ws + li_ws_a(M, N, K));
+    float *scale = (float *)(ws + li_ws_scale(M, N, K));
+    A.a = codes;
+    A.a_scale = scale;
+    int rc = frcnn_i8_quantize(x, x_type, x_stride, M, K, n_rows, codes, li_stride(K), scale, st);
+    if (rc == FRCNN_OK) rc = li_in_rows(&A.b, &A.b_stride, N, K, ws + li_ws_b(M, N, K), st);
+    return rc == FRCNN_OK ? li_launch<1>(A, p, ws, st) : rc;
 }
 
 // Workspace of the gradients: for dL/dx the digits (3, M, N), their magnitudes, b transposed (K, N) and the sums of a
 // split; for dL/dw the digits (3, N, M), magnitudes, column partials, a transposed (K, M) and the sums of a split.
 struct LiGrad {
-    size_t digits, top, col_sum, partials, other, split, total;
+    size_t digits, top, partials, other, split, total;
     LiPlan plan;
 };
 
@@ -479,12 +846,11 @@ static LiGrad li_grad_plan(int rows, int cols, int inner, size_t partials)
     const size_t ld = (size_t)li_stride(inner);
     size_t off = 0;
     g.plan = li_plan(rows, cols, inner, 3);
+    g.split = off; off += up256(li_split_bytes(g.plan, rows, cols, 3));
     g.digits = off; off += up256(3 * (size_t)rows * ld);
     g.top = off; off += up256((size_t)rows * 4);
-    g.col_sum = off; off += up256((size_t)rows * 4);
     g.partials = off; off += up256(partials);
     g.other = off; off += up256((size_t)cols * ld);
-    g.split = off; off += li_partial_bytes(g.plan, rows, cols, 3);
     g.total = off;
     return g;
 }
@@ -515,40 +881,30 @@ extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t
     }
     hipStream_t st = (hipStream_t)stream;
     char *ws = (char *)workspace;
+    int rc = FRCNN_OK;
     if (grad_x) {
         const LiGrad g = li_grad_plan(M, K, N, 0);
         const int64_t ld = li_stride(N), plane = (int64_t)M * ld;
-        int rc = frcnn_i8_grad_row_digits(grad, grad_type, grad_stride, y, y_stride, b_scale, M, N, (int8_t *)(ws + g.digits),
-                                          ld, plane, (float *)(ws + g.top), st);
-        if (rc != FRCNN_OK) return rc;
-        rc = frcnn_i8_transpose(b, b_stride, N, K, (int8_t *)(ws + g.other), ld, st);
-        if (rc != FRCNN_OK) return rc;
-        LiArgs A = {};
-        A.a = (const int8_t *)(ws + g.digits); A.a_stride = ld; A.a_plane = plane;
-        A.b = (const int8_t *)(ws + g.other); A.b_stride = ld;
-        A.M = M; A.N = K; A.K = N;
-        A.a_scale = (const float *)(ws + g.top);
-        A.out = grad_x; A.out_type = grad_x_type; A.out_stride = K;
-        rc = li_launch<3>(A, g.plan, ws + g.split, st);
+        LiArgs A = li_args((int8_t *)(ws + g.digits), ld, (float *)(ws + g.top), (int8_t *)(ws + g.other), ld, nullptr, nullptr,
+                           0, M, K, N, nullptr, grad_x, grad_x_type, K);
+        A.a_plane = plane;
+        rc = frcnn_i8_grad_row_digits(grad, grad_type, grad_stride, y, y_stride, b_scale, M, N, (int8_t *)(ws + g.digits), ld,
+                                      plane, (float *)(ws + g.top), st);
+        if (rc == FRCNN_OK) rc = frcnn_i8_transpose(b, b_stride, N, K, (int8_t *)(ws + g.other), ld, st);
+        if (rc == FRCNN_OK) rc = li_launch<3>(A, g.plan, ws + g.split, st);
         if (rc != FRCNN_OK) return rc;
     }
     if (grad_w || grad_bias) { // the bias gradient is a by-product of the columns' magnitudes
         const LiGrad g = li_grad_plan(N, K, M, frcnn_i8_grad_col_partials(M, N));
         const int64_t ld = li_stride(M), plane = (int64_t)N * ld;
-        int rc = frcnn_i8_grad_col_digits(grad, grad_type, grad_stride, y, y_stride, a_scale, M, N, (int8_t *)(ws + g.digits),
-                                          ld, plane, (float *)(ws + g.top), grad_bias, ws + g.partials, st);
-        if (rc != FRCNN_OK) return rc;
-        if (!grad_w) return FRCNN_OK;
+        LiArgs A = li_args((int8_t *)(ws + g.digits), ld, (float *)(ws + g.top), (int8_t *)(ws + g.other), ld, nullptr, nullptr,
+                           0, N, K, M, nullptr, grad_w, grad_w_type, K);
+        A.a_plane = plane;
+        rc = frcnn_i8_grad_col_digits(grad, grad_type, grad_stride, y, y_stride, a_scale, M, N, (int8_t *)(ws + g.digits), ld,
+                                      plane, (float *)(ws + g.top), grad_bias, ws + g.partials, st);
+        if (!grad_w || rc != FRCNN_OK) return rc;
         rc = frcnn_i8_transpose(a, a_stride, M, K, (int8_t *)(ws + g.other), ld, st);
-        if (rc != FRCNN_OK) return rc;
-        LiArgs A = {};
-        A.a = (const int8_t *)(ws + g.digits); A.a_stride = ld; A.a_plane = plane;
-        A.b = (const int8_t *)(ws + g.other); A.b_stride = ld;
-        A.M = N; A.N = K; A.K = M;
-        A.a_scale = (const float *)(ws + g.top);
-        A.out = grad_w; A.out_type = grad_w_type; A.out_stride = K;
-        rc = li_launch<3>(A, g.plan, ws + g.split, st);
-        if (rc != FRCNN_OK) return rc;
+        if (rc == FRCNN_OK) rc = li_launch<3>(A, g.plan, ws + g.split, st);
     }
-    return FRCNN_OK;
+    return rc;
 }

@@ -1,98 +1,63 @@
 // quantize.hip -- what turns rows of numbers into 8-bit integers for linear_i8.hip: the row quantiser, and for the
 // training step the byte transpose and the digits of the gradients.
-//
-// Row quantiser.  top = max_k |x_k|; scale = top / 127 (fp32); code_k = the whole number nearest to the EXACT quotient
-// 127 x_k / top, ties to even.  Codes do not depend on how a kernel happens to round: 127 x (31 bits) and top (24 bits)
-// are exact in 64-bit floating point, and a quotient of such numbers that is not a half is at least 2^-25 / 2^7 away
-// from it relatively, far more than 2^-53, so one correctly rounded 64-bit division decides.  Almost every code is
-// settled by a 32-bit product instead: t = x * (127 / top) is off by less than 3e-5, so it settles every t that is
-// further than that from a half.
 #include "i8_common.h"
 
-#define QR_NEAR (0.5f - 3.0e-5f)
-
-// The code of x in a row whose largest magnitude is `top`; inv = 127 / top in fp32, or NaN to ask for the division
-// (a top so small that 127 / top leaves fp32).
-__device__ __forceinline__ int qr_code(float x, float top, float inv)
-{
-    const float t = x * inv;
-    const float r = __builtin_rintf(t);
-    if (__builtin_expect(!(fabsf(t - r) < QR_NEAR), 0)) return (int)__builtin_rint((double)x * 127.0 / (double)top);
-    return (int)r;
-}
-
-__device__ __forceinline__ uint32_t qr_pack(int a, int b, int c, int d)
-{
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
-
 // One workgroup a row, the row held in registers between the maximum and the codes (V elements of 16 bytes a load,
-// NV loads a thread), so that x is read once.  A row with an Inf or a NaN has scale NaN and codes 0: products of it
-// are NaN, never a plausible number.
+// NV loads a thread), so that x is read once.
+// Two workgroups' rows have to fit a CU, so that one loads while the other computes: registers are bounded to 64.
 template <typename T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 8)
 quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride, int M, int K, const int32_t *__restrict__ n_rows,
                      int8_t *__restrict__ codes, int64_t c_stride, float *__restrict__ scale)
 {
     constexpr int V = 16 / sizeof(T);
     __shared__ uint32_t red[THREADS / 64];
-    const int row = blockIdx.x;
+    const int row = blockIdx.x, t = threadIdx.x;
     if (row >= i8_rows(n_rows, M)) return;
     const T *xr = x + (int64_t)row * x_stride;
     int8_t *cr = codes + (int64_t)row * c_stride;
+    const int kf = K - K % V; // whole vectors up to here; the last K % V elements one a thread
     I8Vec<T, V> v[NV];
-    uint32_t top_bits = 0; // magnitudes as integers: order kept, Inf above every number and NaN above Inf
+    T v_tail = kf + t < K && t < V ? xr[kf + t] : (T)0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int k = (i * THREADS + (int)threadIdx.x) * V;
-        if (k + V <= K) {
-            v[i] = i8_load<T, V>(xr + k);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) v[i].v[j] = k + j < K ? xr[k + j] : (T)0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const uint32_t m = __float_as_uint((float)v[i].v[j]) & 0x7fffffffu;
-            top_bits = m > top_bits ? m : top_bits;
-        }
+        const int k = (i * THREADS + t) * V;
+        v[i] = I8Vec<T, V>{};
+        if (k < kf) v[i] = i8_load<T, V>(xr + k);
     }
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t m = __shfl_xor(top_bits, o);
-        top_bits = m > top_bits ? m : top_bits;
-    }
-    if (THREADS > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top_bits;
-        __syncthreads();
+    uint32_t top_bits = qr_bits((float)v_tail);
 #pragma unroll
-        for (int w = 0; w < THREADS / 64; ++w) top_bits = red[w] > top_bits ? red[w] : top_bits;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) top_bits = qr_max(top_bits, qr_bits((float)v[i].v[j]));
+    const QrRow q = qr_row(qr_block_max<THREADS>(top_bits, red));
+    if (t == 0) scale[row] = q.scale;
+    if (__builtin_expect(q.far, 0)) {
+        v_tail = qr_lift(v_tail, q);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i].v[j] = qr_lift(v[i].v[j], q);
     }
-    const bool finite = top_bits < 0x7f800000u;
-    const float top = __uint_as_float(top_bits);
-    const bool none = !finite || top_bits == 0;
-    const float inv = none ? 0.0f : (top < 1e-30f ? __builtin_nanf("") : 127.0f / top);
-    if (threadIdx.x == 0) scale[row] = finite ? top / 127.0f : __builtin_nanf("");
-    // the stride is a multiple of 16 whenever K is not: bytes up to the next multiple belong to the row
-    const int kp = (K + 15) & ~15;
     const bool wide = (c_stride & 15) == 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int k = (i * THREADS + (int)threadIdx.x) * V;
-        if (k >= (wide ? kp : K)) break;
-        int c[V];
+        const int k = (i * THREADS + t) * V;
+        if (k >= kf) break;
+        uint32_t p[V / 4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) c[j] = none ? 0 : qr_code((float)v[i].v[j], top, inv);
-        if (wide) {
-            uint32_t p[V / 4];
+        for (int j = 0; j < V / 4; ++j) {
+            int c[4];
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) p[j] = qr_pack(c[4 * j], c[4 * j + 1], c[4 * j + 2], c[4 * j + 3]);
-            __builtin_memcpy(__builtin_assume_aligned(cr + k, V), p, V);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (k + j < K) cr[k + j] = (int8_t)c[j];
+            for (int e = 0; e < 4; ++e) c[e] = q.none ? 0 : qr_code((float)v[i].v[4 * j + e], q);
+            p[j] = qr_pack(c[0], c[1], c[2], c[3]);
         }
+        if (wide) __builtin_memcpy(__builtin_assume_aligned(cr + k, V), p, V);
+        else __builtin_memcpy(cr + k, p, V);
     }
+    // the tail, and with a stride that is a multiple of 16 zeros up to the next multiple, which belong to the row
+    if (t < 16 && kf + t < (wide ? (K + 15) & ~15 : K))
+        cr[kf + t] = (int8_t)(q.none || kf + t >= K ? 0 : qr_code((float)v_tail, q));
 }
 
 // Rows too long for the registers of a workgroup: the same in two passes over the row.
@@ -107,24 +72,12 @@ quantize_rows_long_kernel(const T *__restrict__ x, int64_t x_stride, int M, int 
     const T *xr = x + (int64_t)row * x_stride;
     int8_t *cr = codes + (int64_t)row * c_stride;
     uint32_t top_bits = 0;
-    for (int k = threadIdx.x; k < K; k += 1024) {
-        const uint32_t m = __float_as_uint((float)xr[k]) & 0x7fffffffu;
-        top_bits = m > top_bits ? m : top_bits;
-    }
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t m = __shfl_xor(top_bits, o);
-        top_bits = m > top_bits ? m : top_bits;
-    }
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top_bits;
-    __syncthreads();
-    for (int w = 0; w < 16; ++w) top_bits = red[w] > top_bits ? red[w] : top_bits;
-    const bool finite = top_bits < 0x7f800000u;
-    const float top = __uint_as_float(top_bits);
-    const bool none = !finite || top_bits == 0;
-    const float inv = none ? 0.0f : (top < 1e-30f ? __builtin_nanf("") : 127.0f / top);
-    if (threadIdx.x == 0) scale[row] = finite ? top / 127.0f : __builtin_nanf("");
-    const int kp = (c_stride & 15) == 0 ? (K + 15) & ~15 : K;
-    for (int k = threadIdx.x; k < kp; k += 1024) cr[k] = (int8_t)(none || k >= K ? 0 : qr_code((float)xr[k], top, inv));
+    for (int k = threadIdx.x; k < K; k += 1024) top_bits = qr_max(top_bits, qr_bits((float)xr[k]));
+    const QrRow q = qr_row(qr_block_max<1024>(top_bits, red));
+    if (threadIdx.x == 0) scale[row] = q.scale;
+    const int end = (c_stride & 15) == 0 ? (K + 15) & ~15 : K;
+    for (int k = threadIdx.x; k < end; k += 1024)
+        cr[k] = (int8_t)(q.none || k >= K ? 0 : qr_code((float)(q.far ? qr_lift(xr[k], q) : xr[k]), q));
 }
 
 template <typename T>
@@ -139,15 +92,35 @@ static int quantize_rows_t(const T *x, int64_t x_stride, int M, int K, const int
         FRCNN_CHECK_LAUNCH("quantize_rows");                                                                        \
         return FRCNN_OK;                                                                                            \
     }
-    QR_LAUNCH(64, 4)
-    QR_LAUNCH(256, 4)
-    QR_LAUNCH(256, 16)
-    QR_LAUNCH(512, 16)
+    // four loads a thread, or one where there are too few rows to fill the chip
+    if (M >= 1024) {
+        QR_LAUNCH(64, 4)
+        QR_LAUNCH(128, 4)
+        QR_LAUNCH(256, 4)
+        QR_LAUNCH(512, 4)
+    }
+    QR_LAUNCH(64, 1)
+    QR_LAUNCH(256, 1)
+    QR_LAUNCH(1024, 1)
+    QR_LAUNCH(1024, 4)
+    if constexpr (V == 4) {
+        QR_LAUNCH(1024, 7) // what 64 registers hold
+    }
 #undef QR_LAUNCH
     hipLaunchKernelGGL((quantize_rows_long_kernel<T>), dim3(M), dim3(1024), 0, st, x, x_stride, M, K, n_rows, codes,
                        c_stride, scale);
     FRCNN_CHECK_LAUNCH("quantize_rows");
     return FRCNN_OK;
+}
+
+int frcnn_i8_quantize(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows, int8_t *codes,
+                      int64_t codes_stride, float *scale, hipStream_t st)
+{
+    if (x_type == FRCNN_F32)
+        return quantize_rows_t((const float *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
+    if (x_type == FRCNN_BF16)
+        return quantize_rows_t((const __bf16 *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
+    return quantize_rows_t((const _Float16 *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
 }
 
 extern "C" int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows,
@@ -160,12 +133,7 @@ extern "C" int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_strid
     FRCNN_REQUIRE(x && codes && scale, "quantize_rows: null pointer");
     FRCNN_REQUIRE((codes_stride & 15) != 0 || ((uintptr_t)codes & 15) == 0,
                   "quantize_rows: codes of a padded row stride have to be 16-byte aligned");
-    hipStream_t st = (hipStream_t)stream;
-    if (x_type == FRCNN_F32)
-        return quantize_rows_t((const float *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
-    if (x_type == FRCNN_BF16)
-        return quantize_rows_t((const __bf16 *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
-    return quantize_rows_t((const _Float16 *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
+    return frcnn_i8_quantize(x, x_type, x_stride, M, K, n_rows, codes, codes_stride, scale, (hipStream_t)stream);
 }
 
 // ---- rows copied to an aligned row stride -----------------------------------------------------------------------
@@ -245,8 +213,9 @@ template <typename T> __device__ __forceinline__ float gd_grad(const T *grad, co
 // formed in 64 bits.
 __device__ __forceinline__ int gd_fix(float a, double inv) { return (int)__builtin_rint((double)a * inv); }
 
-// For dL/dx: a_mn = g_mn * col_scale_n, fixed point relative to the row's largest magnitude.  One wave a row.
-template <typename T>
+// For dL/dx: a_mn = g_mn * col_scale_n, fixed point relative to the row's largest magnitude.  One wave a row, four
+// neighbours a lane, up to NV of those held in registers; a longer row is read again (from the caches) for its digits.
+template <typename T, int NV>
 __global__ void __launch_bounds__(256)
 grad_row_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__restrict__ y, int64_t y_stride,
                        const float *__restrict__ col_scale, int M, int N, int8_t *__restrict__ digits, int64_t stride,
@@ -255,34 +224,54 @@ grad_row_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= M) return;
+    const T *g = grad + row * g_stride, *z = y ? y + row * y_stride : nullptr;
+    auto load = [&](float(&a)[4], int n) {
+        if (n + 4 <= N) {
+            const I8Vec<T, 4> v = i8_load<T, 4>(g + n);
+            const I8Vec<float, 4> c = i8_load<float, 4>(col_scale + n);
+            I8Vec<T, 4> u = v;
+            if (z) u = i8_load<T, 4>(z + n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = (z && (float)u.v[j] <= 0.0f ? 0.0f : (float)v.v[j]) * c.v[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = n + j < N ? gd_grad(g, z, n + j, n + j) * col_scale[n + j] : 0.0f;
+        }
+    };
+    float a[NV][4];
     uint32_t top_bits = 0;
-    for (int n = lane; n < N; n += 64) {
-        const float a = gd_grad(grad, y, row * g_stride + n, row * y_stride + n) * col_scale[n];
-        const uint32_t m = __float_as_uint(a) & 0x7fffffffu;
-        top_bits = m > top_bits ? m : top_bits;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load(a[i], (i * 64 + lane) * 4);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top_bits = qr_max(top_bits, qr_bits(a[i][j]));
+    for (int n = (NV * 64 + lane) * 4; n < N; n += 256) {
+        float t[4];
+        load(t, n);
+        for (int j = 0; j < 4; ++j) top_bits = qr_max(top_bits, qr_bits(t[j]));
     }
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t m = __shfl_xor(top_bits, o);
-        top_bits = m > top_bits ? m : top_bits;
-    }
+    for (int o = 32; o > 0; o >>= 1) top_bits = qr_max(top_bits, __shfl_xor(top_bits, o));
     const bool finite = top_bits < 0x7f800000u;
     const float top = __uint_as_float(top_bits);
-    const double inv = !finite || top_bits == 0 ? 0.0 : (double)I8_FIX / (double)top;
+    const bool none = !finite || top_bits == 0;
+    const double inv = none ? 0.0 : (double)I8_FIX / (double)top;
     if (lane == 0) row_top[row] = finite ? top : __builtin_nanf("");
     int8_t *d = digits + row * stride;
-    for (int n = lane * 4; n < (int)stride; n += 256) {
-        uint32_t w[3] = {0, 0, 0};
-        for (int j = 0; j < 4; ++j) {
-            if (n + j < N && inv != 0.0) {
-                const float a = gd_grad(grad, y, row * g_stride + n + j, row * y_stride + n + j) * col_scale[n + j];
-                int d0, d1, d2;
-                i8_digits(gd_fix(a, inv), d0, d1, d2);
-                w[0] |= (uint32_t)(d0 & 255) << (8 * j);
-                w[1] |= (uint32_t)(d1 & 255) << (8 * j);
-                w[2] |= (uint32_t)(d2 & 255) << (8 * j);
-            }
-        }
-        for (int p = 0; p < 3; ++p) *(uint32_t *)(d + p * plane + n) = w[p];
+    auto store = [&](const float(&t)[4], int n) {
+        int q[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) i8_digits(none ? 0 : gd_fix(t[j], inv), q[0][j], q[1][j], q[2][j]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *(uint32_t *)(d + p * plane + n) = qr_pack(q[p][0], q[p][1], q[p][2], q[p][3]);
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if ((i * 64 + lane) * 4 < (int)stride) store(a[i], (i * 64 + lane) * 4);
+    for (int n = (NV * 64 + lane) * 4; n < (int)stride; n += 256) {
+        float t[4];
+        load(t, n);
+        store(t, n);
     }
 }
 
@@ -291,8 +280,14 @@ int frcnn_i8_grad_row_digits(const void *grad, int type, int64_t grad_stride, co
                              float *row_top, hipStream_t stream)
 {
 #define GR_LAUNCH(T)                                                                                                    \
-    hipLaunchKernelGGL((grad_row_digits_kernel<T>), dim3((M + 3) / 4), dim3(256), 0, stream, (const T *)grad, grad_stride, \
-                       (const T *)y, y_stride, col_scale, M, N, digits, stride, plane, row_top)
+    do {                                                                                                                \
+        if (N <= 256)                                                                                                   \
+            hipLaunchKernelGGL((grad_row_digits_kernel<T, 1>), dim3((M + 3) / 4), dim3(256), 0, stream, (const T *)grad, \
+                               grad_stride, (const T *)y, y_stride, col_scale, M, N, digits, stride, plane, row_top);   \
+        else                                                                                                            \
+            hipLaunchKernelGGL((grad_row_digits_kernel<T, 4>), dim3((M + 3) / 4), dim3(256), 0, stream, (const T *)grad, \
+                               grad_stride, (const T *)y, y_stride, col_scale, M, N, digits, stride, plane, row_top);   \
+    } while (0)
     if (type == FRCNN_F32) GR_LAUNCH(float);
     else if (type == FRCNN_BF16) GR_LAUNCH(__bf16);
     else GR_LAUNCH(_Float16);
@@ -305,7 +300,7 @@ int frcnn_i8_grad_row_digits(const void *grad, int type, int64_t grad_stride, co
 // (n, m).  First pass: largest magnitude and plain sum (dL/dbias) of every column over GC_ROWS rows; second pass: the
 // column's magnitude from those partials, the digits, and the sum of the partials in row order (the same bits every
 // run).
-#define GC_ROWS 256
+#define GC_ROWS 64
 template <typename T>
 __global__ void __launch_bounds__(256)
 grad_col_partials_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__restrict__ y, int64_t y_stride,
@@ -320,13 +315,17 @@ grad_col_partials_kernel(const T *__restrict__ grad, int64_t g_stride, const T *
     uint32_t top = 0;
     float sum = 0.0f;
     if (n < N) {
-        for (int i = wave; i < GC_ROWS; i += 4) {
-            const int64_t m = m0 + i;
-            if (m >= M) break;
-            const float g = gd_grad(grad, y, m * g_stride + n, m * y_stride + n);
-            const uint32_t b = __float_as_uint(g * row_scale[m]) & 0x7fffffffu;
-            top = b > top ? b : top;
-            sum += g;
+        float g[GC_ROWS / 4], s[GC_ROWS / 4]; // all loads before the first use
+#pragma unroll
+        for (int i = 0; i < GC_ROWS / 4; ++i) {
+            const int64_t m = m0 + i * 4 + wave;
+            g[i] = m < M ? gd_grad(grad, y, m * g_stride + n, m * y_stride + n) : 0.0f;
+            s[i] = m < M ? row_scale[m] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < GC_ROWS / 4; ++i) {
+            top = qr_max(top, qr_bits(g[i] * s[i]));
+            sum += g[i];
         }
     }
     tops[wave][lane] = top;
@@ -358,9 +357,9 @@ grad_col_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
         uint32_t top = 0;
         float sum = 0.0f;
         if (n < N) {
+#pragma unroll 16
             for (int p = 0; p < n_part; ++p) {
-                const uint32_t b = part_top[(int64_t)p * N + n];
-                top = b > top ? b : top;
+                top = qr_max(top, part_top[(int64_t)p * N + n]);
                 sum += part_sum[(int64_t)p * N + n];
             }
         }
@@ -375,14 +374,20 @@ grad_col_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = n0 + lane;
     const double inv = inv_s[lane];
-    for (int i = wave; i < 64; i += 4) {
-        const int64_t m = m0 + i;
-        int d0 = 0, d1 = 0, d2 = 0;
-        if (m < M && n < N && inv != 0.0)
-            i8_digits(gd_fix(gd_grad(grad, y, m * g_stride + n, m * y_stride + n) * row_scale[m], inv), d0, d1, d2);
-        tile[0][lane][i] = (int8_t)d0;
-        tile[1][lane][i] = (int8_t)d1;
-        tile[2][lane][i] = (int8_t)d2;
+    float a[16]; // rows 16 wave .. 16 wave + 15 of the tile
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t m = m0 + wave * 16 + i;
+        a[i] = m < M && n < N ? gd_grad(grad, y, m * g_stride + n, m * y_stride + n) * row_scale[m] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int q[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) i8_digits(inv != 0.0 ? gd_fix(a[4 * i + j], inv) : 0, q[0][j], q[1][j], q[2][j]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            *(uint32_t *)&tile[p][lane][wave * 16 + 4 * i] = qr_pack(q[p][0], q[p][1], q[p][2], q[p][3]);
     }
     __syncthreads();
     const int tn = threadIdx.x >> 2, tm = (threadIdx.x & 3) * 16;

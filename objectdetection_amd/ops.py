@@ -11,6 +11,7 @@ imports those two names (RPN/rpn.py:18, ROIHead/roi_head.py:26, ROIHead/roi_pool
 """
 import collections
 import ctypes
+import functools
 import os
 import math
 
@@ -982,16 +983,49 @@ class MultiScaleRoIAlign(torch.nn.Module):
 _I8_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 I8_MAX_K = 131071  # the 32-bit sums of the product cannot wrap up to here
 
+# A layer of a few rows is bound by the host, so these wrappers spend little there: pointers go to ctypes as numbers, the
+# stream comes as a number without a Stream object around it (0.1 us against 1.9), the device is switched only if it is
+# another one, and tensors that already have the right form are not touched.
+
+
+def _i8_call(name, dev, *args):
+    """One entry point on dev's current stream."""
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _i8_workspace_bytes(name, M, N, K):
+    return max(getattr(_lib.load(), name)(M, N, K), 16)
+
+
+def _at(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _i8_device(what, dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device != dev:
+            _need_gpu(t)
+            raise ValueError("%s: all tensors have to be on %s; got one on %s" % (what, dev, t.device))
+
 
 def _i8_rows(x, what):
     """x (M,K) as a tensor the kernels read in place: one of the three float types, elements of a row next to each
     other, rows any stride apart."""
+    if not x.is_cuda:
+        _need_gpu(x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError("%s expects (M,K) with K > 0; got %s" % (what, tuple(x.shape)))
-    x = x.detach()
     if x.dtype not in _I8_TYPES:
-        x = x.to(torch.float32)
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+        x = x.detach().to(torch.float32)
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.detach().contiguous()
 
 
 def _row_stride(t):
@@ -999,26 +1033,34 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _i8_count(n_rows):
+def _i8_codes(codes):
+    return codes if codes.stride(1) == 1 or codes.shape[1] == 1 else codes.contiguous()
+
+
+def _f32v(t):
+    """A vector as the kernels read it."""
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else t.detach().to(torch.float32).contiguous()
+
+
+def _i8_count(n_rows, what, dev):
     if n_rows is None:
         return None
+    _i8_device(what, dev, n_rows)
     if n_rows.numel() != 1:
-        raise ValueError("n_rows expects one element; got %s" % (tuple(n_rows.shape),))
+        raise ValueError("%s: n_rows expects one element; got %s" % (what, tuple(n_rows.shape)))
     return n_rows if n_rows.dtype == torch.int32 else n_rows.to(torch.int32)
 
 
 def _i8_weights(codes, scale, bias, K, dev, what):
+    _i8_device(what, dev, codes, scale, bias)
     if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[0] == 0 or codes.shape[1] != K:
         raise ValueError("%s expects weight codes (N,%d) int8; got %s %s" % (what, K, tuple(codes.shape), codes.dtype))
     N = codes.shape[0]
-    if scale.shape != (N,) or (bias is not None and bias.shape != (N,)):
+    if scale.dim() != 1 or scale.shape[0] != N or (bias is not None and (bias.dim() != 1 or bias.shape[0] != N)):
         raise ValueError("%s expects a scale and a bias for each of the %d outputs" % (what, N))
     if K > I8_MAX_K:
         raise ValueError("%s: rows of %d; at most %d" % (what, K, I8_MAX_K))
-    if codes.device != dev or scale.device != dev or (bias is not None and bias.device != dev):
-        raise ValueError("%s: all tensors have to be on %s" % (what, dev))
-    codes = codes if codes.stride(1) == 1 or K == 1 else codes.contiguous()
-    return N, codes, _f32c(scale), _f32c(bias) if bias is not None else None
+    return N, _i8_codes(codes), _f32v(scale), _f32v(bias)
 
 
 def quantize_rows_i8(x, n_rows=None):
@@ -1027,24 +1069,22 @@ def quantize_rows_i8(x, n_rows=None):
     A row of zeros: scale 0, codes 0; a row with an Inf or a NaN: scale NaN, codes 0.  n_rows (1) int32 on the device:
     rows behind it are left out (their outputs are unspecified), as in the padded RoI path.  Rows of the codes lie a
     multiple of 16 bytes apart, the form matmul_i8 reads in place."""
-    _need_gpu(x, n_rows)
     x = _i8_rows(x, "quantize_rows_i8")
-    n_rows = _i8_count(n_rows)
     M, K = x.shape
+    dev = x.device
+    n_rows = _i8_count(n_rows, "quantize_rows_i8", dev)
     kp = (K + 15) // 16 * 16
-    codes = torch.empty((M, kp), dtype=torch.int8, device=x.device)
-    scale = torch.empty((M,), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = _lib.load().frcnn_quantize_rows_i8(_ptr(x), _I8_TYPES[x.dtype], _row_stride(x), M, K, _ptr(n_rows),
-                                                _ptr(codes), kp, _ptr(scale), _stream())
-    _lib.check(rc, "quantize_rows_i8")
+    codes = torch.empty((M, kp), dtype=torch.int8, device=dev)
+    scale = torch.empty((M,), dtype=torch.float32, device=dev)
+    _i8_call("frcnn_quantize_rows_i8", dev, x.data_ptr(), _I8_TYPES[x.dtype], _row_stride(x), M, K, _at(n_rows),
+             codes.data_ptr(), kp, scale.data_ptr())
     return (codes if kp == K else codes[:, :K]), scale
 
 
 def matmul_i8(codes, scale, weight_codes, weight_scale, bias=None, relu=False, out_dtype=torch.float32, n_rows=None):
     """out (M,N) = (codes @ weight_codes^T) * scale[:, None] * weight_scale + bias, then max(., 0) if relu: the product
     of two row-quantised matrices (quantize_rows_i8), its sums exact, the rest in 64 bits, rounded to out_dtype."""
-    _need_gpu(codes, scale, weight_codes, weight_scale, bias, n_rows)
+    _need_gpu(codes, scale)
     if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] == 0 or scale.shape != (codes.shape[0],):
         raise ValueError("matmul_i8 expects codes (M,K) int8 and a scale for each row; got %s %s, %s"
                          % (tuple(codes.shape), codes.dtype, tuple(scale.shape)))
@@ -1052,20 +1092,15 @@ def matmul_i8(codes, scale, weight_codes, weight_scale, bias=None, relu=False, o
         raise ValueError("matmul_i8: out_dtype is float32, bfloat16 or float16; got %s" % out_dtype)
     M, K = codes.shape
     dev = codes.device
-    if scale.device != dev or (n_rows is not None and n_rows.device != dev):
-        raise ValueError("matmul_i8: all tensors have to be on %s" % dev)
+    _i8_device("matmul_i8", dev, scale)
     N, weight_codes, weight_scale, bias = _i8_weights(weight_codes, weight_scale, bias, K, dev, "matmul_i8")
-    codes = codes if codes.stride(1) == 1 or K == 1 else codes.contiguous()
-    scale, n_rows = _f32c(scale), _i8_count(n_rows)
+    codes, scale, n_rows = _i8_codes(codes), _f32v(scale), _i8_count(n_rows, "matmul_i8", dev)
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    lib = _lib.load()
-    nbytes = lib.frcnn_matmul_i8_workspace_bytes(M, N, K)
-    ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.frcnn_matmul_i8(_ptr(codes), _row_stride(codes), _ptr(scale), _ptr(weight_codes),
-                                 _row_stride(weight_codes), _ptr(weight_scale), _ptr(bias), int(bool(relu)), M, N, K,
-                                 _ptr(n_rows), _ptr(out), _I8_TYPES[out_dtype], N, _ptr(ws), nbytes, _stream())
-    _lib.check(rc, "matmul_i8")
+    nbytes = _i8_workspace_bytes("frcnn_matmul_i8_workspace_bytes", M, N, K)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _i8_call("frcnn_matmul_i8", dev, codes.data_ptr(), _row_stride(codes), scale.data_ptr(), weight_codes.data_ptr(),
+             _row_stride(weight_codes), weight_scale.data_ptr(), _at(bias), 1 if relu else 0, M, N, K, _at(n_rows),
+             out.data_ptr(), _I8_TYPES[out_dtype], N, ws.data_ptr(), nbytes)
     return out
 
 
@@ -1074,26 +1109,21 @@ def linear_i8(x, weight_codes, weight_scale, bias=None, relu=False, out_dtype=No
     (N,K) int8 and weight_scale (N) from quantize_rows_i8(weight); -> (M,N) in out_dtype (x's type by default).
     n_rows (1) int32 on the device: rows behind it are neither read nor written.  The result is detached; LinearI8 is
     the differentiable form."""
-    _need_gpu(x, weight_codes, weight_scale, bias, n_rows)
     x = _i8_rows(x, "linear_i8")
     M, K = x.shape
     dev = x.device
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _I8_TYPES:
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype not in _I8_TYPES:
         raise ValueError("linear_i8: out_dtype is float32, bfloat16 or float16; got %s" % out_dtype)
-    if n_rows is not None and n_rows.device != dev:
-        raise ValueError("linear_i8: all tensors have to be on %s" % dev)
     N, weight_codes, weight_scale, bias = _i8_weights(weight_codes, weight_scale, bias, K, dev, "linear_i8")
-    n_rows = _i8_count(n_rows)
+    n_rows = _i8_count(n_rows, "linear_i8", dev)
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    lib = _lib.load()
-    nbytes = lib.frcnn_linear_i8_workspace_bytes(M, N, K)
-    ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.frcnn_linear_i8(_ptr(x), _I8_TYPES[x.dtype], _row_stride(x), _ptr(weight_codes),
-                                 _row_stride(weight_codes), _ptr(weight_scale), _ptr(bias), int(bool(relu)), M, N, K,
-                                 _ptr(n_rows), _ptr(out), _I8_TYPES[out_dtype], N, _ptr(ws), nbytes, _stream())
-    _lib.check(rc, "linear_i8")
+    nbytes = _i8_workspace_bytes("frcnn_linear_i8_workspace_bytes", M, N, K)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _i8_call("frcnn_linear_i8", dev, x.data_ptr(), _I8_TYPES[x.dtype], _row_stride(x), weight_codes.data_ptr(),
+             _row_stride(weight_codes), weight_scale.data_ptr(), _at(bias), 1 if relu else 0, M, N, K, _at(n_rows),
+             out.data_ptr(), _I8_TYPES[out_dtype], N, ws.data_ptr(), nbytes)
     return out
 
 
@@ -1102,39 +1132,34 @@ def linear_i8_backward(grad, y, codes, scale, weight_codes, weight_scale, x_dtyp
     """Straight-through gradients of matmul_i8 (rounding counts as the identity): grad (M,N) = dL/dout in y's type, y
     the layer's output if it ended in a ReLU, else None.  -> (grad_x (M,K), grad_weight (N,K), grad_bias (N) fp32),
     None where not wanted.  Exact sums over 24-bit fixed-point gradients: the same bits every run."""
-    _need_gpu(grad, y, codes, scale, weight_codes, weight_scale)
+    _need_gpu(grad)
     M, K = codes.shape
     N = weight_codes.shape[0]
     dev = grad.device
+    _i8_device("linear_i8_backward", dev, y, codes, scale, weight_codes, weight_scale)
     if grad.shape != (M, N) or (y is not None and (y.shape != (M, N) or y.dtype != grad.dtype)) \
             or weight_codes.shape[1] != K or scale.shape != (M,) or weight_scale.shape != (N,) \
             or codes.dtype != torch.int8 or weight_codes.dtype != torch.int8 or grad.dtype not in _I8_TYPES \
             or x_dtype not in _I8_TYPES or weight_dtype not in _I8_TYPES:
         raise ValueError("linear_i8_backward: inconsistent shapes or types")
-    if any(t is not None and t.device != dev for t in (y, codes, scale, weight_codes, weight_scale)):
-        raise ValueError("linear_i8_backward: all tensors have to be on %s" % dev)
     if M > I8_MAX_K or N > I8_MAX_K or K > I8_MAX_K:
         raise ValueError("linear_i8_backward: (%d, %d, %d); each is at most %d" % (M, N, K, I8_MAX_K))
     if M == 0:
         return (torch.empty((0, K), dtype=x_dtype, device=dev) if want[0] else None,
                 torch.zeros((N, K), dtype=weight_dtype, device=dev) if want[1] else None,
                 torch.zeros((N,), dtype=torch.float32, device=dev) if want[2] else None)
-    grad, y, codes, weight_codes = [t if t is None or t.stride(1) == 1 else t.contiguous()
-                                    for t in (grad.detach(), y, codes, weight_codes)]
-    scale, weight_scale = _f32c(scale), _f32c(weight_scale)
+    grad, codes, weight_codes = _i8_codes(grad), _i8_codes(codes), _i8_codes(weight_codes)
+    y = _i8_codes(y) if y is not None else None
+    scale, weight_scale = _f32v(scale), _f32v(weight_scale)
     gx = torch.empty((M, K), dtype=x_dtype, device=dev) if want[0] else None
     gw = torch.empty((N, K), dtype=weight_dtype, device=dev) if want[1] else None
     gb = torch.empty((N,), dtype=torch.float32, device=dev) if want[2] else None
-    lib = _lib.load()
-    nbytes = lib.frcnn_linear_i8_backward_workspace_bytes(M, N, K)
-    ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        rc = lib.frcnn_linear_i8_backward(
-            _ptr(grad), _I8_TYPES[grad.dtype], _row_stride(grad), _ptr(y), _row_stride(y) if y is not None else 0,
-            _ptr(codes), _row_stride(codes), _ptr(scale), _ptr(weight_codes), _row_stride(weight_codes),
-            _ptr(weight_scale), M, N, K, _ptr(gx), _I8_TYPES[x_dtype], _ptr(gw), _I8_TYPES[weight_dtype], _ptr(gb),
-            _ptr(ws), nbytes, _stream())
-    _lib.check(rc, "linear_i8_backward")
+    nbytes = _i8_workspace_bytes("frcnn_linear_i8_backward_workspace_bytes", M, N, K)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    _i8_call("frcnn_linear_i8_backward", dev, grad.data_ptr(), _I8_TYPES[grad.dtype], _row_stride(grad), _at(y),
+             _row_stride(y) if y is not None else 0, codes.data_ptr(), _row_stride(codes), scale.data_ptr(),
+             weight_codes.data_ptr(), _row_stride(weight_codes), weight_scale.data_ptr(), M, N, K, _at(gx),
+             _I8_TYPES[x_dtype], _at(gw), _I8_TYPES[weight_dtype], _at(gb), ws.data_ptr(), nbytes)
     return gx, gw, gb
 
 
@@ -1162,10 +1187,9 @@ class LinearI8(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        codes, scale, weight_codes, weight_scale = ctx.saved_tensors[:4]
-        y = ctx.saved_tensors[4] if ctx.relu else None
-        gx, gw, gb = linear_i8_backward(grad, y, codes, scale, weight_codes, weight_scale, ctx.types[0], ctx.types[1],
+        saved = ctx.saved_tensors
+        gx, gw, gb = linear_i8_backward(grad, saved[4] if ctx.relu else None, *saved[:4], ctx.types[0], ctx.types[1],
                                         (tuple(ctx.needs_input_grad) + (False,))[:3])
-        if gb is not None:
+        if gb is not None and gb.dtype != ctx.types[2]:
             gb = gb.to(ctx.types[2])
         return gx, gw, gb, None

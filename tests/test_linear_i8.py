@@ -106,9 +106,11 @@ def test_c_entries_refuse_before_any_launch():
     refused(mm(so=3), b"strides")
     refused(mm(a=null), b"null")
     refused(mm(t=9), b"element type")
-    refused(mm(nb=16), b"workspace", -2)
-    refused(mm(ws=null), b"workspace", -2)
-    refused(lib.frcnn_linear_i8(p, 0, 32, p, 32, p, null, 0, 4, 4, 32, null, p, 0, 4, p, 16, null), b"workspace", -2)
+    refused(mm(m=40, nb=16), b"workspace", -2)
+    refused(mm(m=40, ws=null), b"workspace", -2)
+    refused(lib.frcnn_linear_i8(p, 0, 2048, p, 2048, p, null, 0, 40, 4, 2048, null, p, 0, 4, p, 16, null), b"workspace", -2)
+    refused(lib.frcnn_linear_i8(null, 0, 32, p, 32, p, null, 0, 4, 4, 32, null, p, 0, 4, p, 16, null), b"null")
+    refused(lib.frcnn_linear_i8(p, 0, 32, p, 32, p, null, 0, 4, 4, 32, null, p, 0, 3, p, 16, null), b"strides")
     refused(lib.frcnn_linear_i8(p, 7, 32, p, 32, p, null, 0, 4, 4, 32, null, p, 0, 4, p, 1 << 30, null), b"element type")
 
     def bw(m=4, n=4, k=32, a=p, nb=1 << 30):
@@ -323,6 +325,51 @@ def test_linear_i8(dev, m, n, k, dtype):
     same_bits(out, ref)
     if m > 30:
         assert torch.isnan(out[4]).all() and torch.isnan(out[9]).all() and not torch.isnan(out[5]).any()
+
+
+# The three forms (a few rows; short rows, 16 and 64 a workgroup; quantiser and tiles) at the edges between them: rows,
+# channels and lengths beside multiples of 16, 64 and 128, the last weight in the middle of a 16-byte load.
+FORMS = [(1, 1, 15), (2, 7, 17), (4, 5, 4099), (3, 4, 32768), (4, 9, 32769), (5, 3, 16), (3, 1, 16), (16, 16, 31), (17, 15, 33),
+         (15, 129, 63), (64, 2, 65), (65, 105, 127), (100, 257, 1023), (63, 300, 1024), (33, 40, 1025), (130, 128, 1009),
+         (20000, 21, 49), (16500, 130, 48), (17000, 128, 1000), (9000, 300, 80), (5, 513, 1007), (300, 1, 77)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n,k", FORMS)
+def test_linear_i8_forms(dev, m, n, k, dtype):
+    from objectdetection_amd import ops
+    fin = torch.finfo(dtype)
+    x = features(m, k, 3 * m + k, dtype)
+    x[:, 1::2] *= -1
+    # rows at the ends of the type, of ties, with an Inf and a NaN, spread over the workgroups
+    for i, r in enumerate(range(0, m, max(1, m // 9))):
+        if i % 9 == 1:
+            x[r] = (x[r].double() / max(float(x[r].abs().max()), 1e-9) * fin.max).to(dtype)
+        elif i % 9 == 2:
+            x[r] = (x[r].double() * fin.tiny * 0.3).to(dtype)
+        elif i % 9 == 3:
+            x[r] = (torch.arange(k) % 255 - 127).double().mul(0.5).to(dtype)
+            x[r, k // 3] = 127.0
+        elif i % 9 == 4:
+            x[r, k - 1] = float("inf")
+        elif i % 9 == 5:
+            x[r, 0] = float("nan")
+        elif i % 9 == 6:
+            x[r] = 0
+    g = torch.Generator().manual_seed(k)
+    w = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int32).to(torch.int8)
+    ws, bias = torch.rand((n,), generator=g) * 0.01, torch.randn((n,), generator=g)
+    out = ops.linear_i8(x.to(dev), w.to(dev), ws.to(dev), bias.to(dev), True, F32)
+    q, s = plain_codes(x)
+    same_bits(out, plain_product(q, s, w, ws, bias, True, F32))
+    # weight rows on a stride of their own behind an odd offset, rows of x on another, no bias, the type's own output
+    store = torch.zeros((n, k + 13), dtype=torch.int8, device=dev)
+    store[:, 5:5 + k] = w.to(dev)
+    wide = torch.full((m, k + 3), float("nan"), dtype=dtype, device=dev)
+    wide[:, 1:1 + k] = x.to(dev)
+    out = ops.linear_i8(wide[:, 1:1 + k], store[:, 5:5 + k], ws.to(dev))
+    same_bits(out, plain_product(q, s, w, ws, None, False, dtype))
 
 
 # ---------------------------------------------------------------------------------------------------- gradients
