@@ -398,6 +398,18 @@ int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, const int8_t *b
                     void *out, int out_type, int64_t out_stride, void *workspace, size_t workspace_bytes,
                     void *stream);
 
+/* The layer's forward call in training: x (M,K) and w (N,K) are both quantised by rows on every call (the weights change
+ * from step to step) and multiplied as in frcnn_matmul_i8; M > 0.  saved: frcnn_linear_i8_train_saved_bytes(M,N,K) bytes,
+ * 256-byte aligned, for the backward call: with ld = K rounded up to 16 and every part rounded up to 256 bytes, the codes of
+ * x (M, ld), their scales (M), the codes of w (N, ld), their scales (N).  workspace:
+ * frcnn_linear_i8_train_workspace_bytes(M,N,K) bytes, contents need not survive. */
+size_t frcnn_linear_i8_train_saved_bytes(int M, int N, int K);
+size_t frcnn_linear_i8_train_workspace_bytes(int M, int N, int K);
+int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride, const void *w, int w_type, int64_t w_stride,
+                          const float *bias, int relu, int M, int N, int K, void *out, int out_type,
+                          int64_t out_stride, void *saved, size_t saved_bytes, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
 /* Straight-through gradients of the layer (rounding counts as the identity), from grad = dL/dout (M,N) and the codes
  * and scales of the forward call.  g = grad, or 0 where y <= 0 (y: the forward's output in grad's type if it ended in
  * a ReLU, NULL otherwise):

@@ -69,6 +69,9 @@ SIGNATURES = {
     "frcnn_matmul_i8": (_I, [_P, _L, _P, _P, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _L, _P, _Z, _P]),
     "frcnn_linear_i8_workspace_bytes": (_Z, [_I, _I, _I]),
     "frcnn_linear_i8": (_I, [_P, _I, _L, _P, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _L, _P, _Z, _P]),
+    "frcnn_linear_i8_train_saved_bytes": (_Z, [_I, _I, _I]),
+    "frcnn_linear_i8_train_workspace_bytes": (_Z, [_I, _I, _I]),
+    "frcnn_linear_i8_train": (_I, [_P, _I, _L, _P, _I, _L, _P, _I, _I, _I, _I, _P, _I, _L, _P, _Z, _P, _Z, _P]),
     "frcnn_linear_i8_backward_workspace_bytes": (_Z, [_I, _I, _I]),
     "frcnn_linear_i8_backward": (_I, [_P, _I, _L, _P, _L, _P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _I, _P, _I, _P, _P, _Z,
                                       _P]),

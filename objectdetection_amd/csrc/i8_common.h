@@ -110,17 +110,42 @@ __device__ __forceinline__ void i8_digits(int T, int &d0, int &d1, int &d2)
 // Longest contraction: 2^17 - 1 products of at most 2^14 cannot leave 32 bits.
 #define I8_MAX_K 131071
 
-// quantize.hip, used by linear_i8.hip
-int frcnn_i8_quantize(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows, int8_t *codes,
-                      int64_t codes_stride, float *scale, hipStream_t stream);
+// ---- quantize.hip, used by linear_i8.hip ---------------------------------------------------------------------------
+struct I8Rows { // rows to quantise, and where to
+    const void *x;
+    int type;
+    int64_t x_stride;
+    int M;
+    const int32_t *n_rows;
+    int8_t *codes;
+    int64_t c_stride;
+    float *scale;
+};
+// A and, in the same launch where it is of the same type, B (B.M = 0: none)
+int frcnn_i8_quantize(const I8Rows &A, const I8Rows &B, int K, hipStream_t stream);
 int frcnn_i8_pad_rows(const int8_t *src, int64_t src_stride, int rows, int K, int8_t *dst, int64_t dst_stride,
                       hipStream_t stream);
-int frcnn_i8_transpose(const int8_t *src, int64_t src_stride, int rows, int cols, int8_t *dst, int64_t dst_stride,
-                       hipStream_t stream);
-int frcnn_i8_grad_row_digits(const void *grad, int type, int64_t grad_stride, const void *y, int64_t y_stride,
-                             const float *col_scale, int M, int N, int8_t *digits, int64_t stride, int64_t plane,
-                             float *row_top, hipStream_t stream);
-size_t frcnn_i8_grad_col_partials(int M, int N);
-int frcnn_i8_grad_col_digits(const void *grad, int type, int64_t grad_stride, const void *y, int64_t y_stride,
-                             const float *row_scale, int M, int N, int8_t *digits, int64_t stride, int64_t plane,
-                             float *col_top, float *col_sum, void *partials, hipStream_t stream);
+
+struct I8Grad { // a training step's backward inputs, and what its products read
+    const void *grad, *y; // y NULL: no ReLU
+    int type;
+    int64_t grad_stride, y_stride;
+    const int8_t *a, *b;
+    int64_t a_stride, b_stride;
+    const float *a_scale, *b_scale;
+    int M, N, K;
+    // dL/dx: digits (3, M, row_stride) of g b_scale, their magnitudes (M), b transposed (K, row_stride); NULL: not wanted
+    int8_t *row_digits, *b_t;
+    float *row_top;
+    int64_t row_stride;
+    // dL/dw: digits (3, N, col_stride) of g a_scale, their magnitudes (N), a transposed (K, col_stride; NULL: only
+    // dL/dbias wanted), partial magnitudes and sums of the columns (frcnn_i8_grad_parts(M), N)
+    int8_t *col_digits, *a_t;
+    float *col_top;
+    int64_t col_stride;
+    uint32_t *part_top;
+    float *part_sum;
+    float *grad_bias;
+};
+int frcnn_i8_grad_parts(int M);
+int frcnn_i8_grad_prepare(const I8Grad &A, hipStream_t stream);

@@ -77,11 +77,11 @@ __device__ __forceinline__ int li_swz(int r) { return (-(r >> 2)) & 3; }
 
 // Workgroups go to the eight XCDs in turn: neighbours in the tile order go to one XCD, eight tiles of m by all of n, so
 // that its L2 sees a row of a and a row of b several times.
-__device__ __forceinline__ void li_tile(int tiles_m, int tiles_n, int &tm, int &tn)
+__device__ __forceinline__ void li_tile(int block, int tiles_m, int tiles_n, int &tm, int &tn)
 {
     const int tiles = tiles_m * tiles_n;
-    const int xcd = blockIdx.x & 7, q = tiles >> 3, r = tiles & 7;
-    const int l = xcd * q + (xcd < r ? xcd : r) + (blockIdx.x >> 3);
+    const int xcd = block & 7, q = tiles >> 3, r = tiles & 7;
+    const int l = xcd * q + (xcd < r ? xcd : r) + (block >> 3);
     const int group = l / (8 * tiles_n), rem = l - group * 8 * tiles_n;
     const int gm = tiles_m - group * 8 < 8 ? tiles_m - group * 8 : 8;
     tm = group * 8 + rem % gm;
@@ -91,7 +91,7 @@ __device__ __forceinline__ void li_tile(int tiles_m, int tiles_n, int &tm, int &
 // One tile of BM x BN by waves of WM x WN.  k goes by in stages of 64 bytes: global -> LDS directly, LI_STAGES in the
 // ring; LDS -> registers one stage ahead of the matrix instructions; so that a load has LI_STAGES - 1 stages to arrive.
 template <int BM, int BN, int WM, int WN, int P>
-__device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
+__device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int split)
 {
     constexpr int BK = LI_BK;
     constexpr int NW = (BM / WM) * (BN / WN);
@@ -109,11 +109,11 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tile_m, tile_n;
-    li_tile(A.tiles_m, A.tiles_n, tile_m, tile_n);
+    li_tile(block, A.tiles_m, A.tiles_n, tile_m, tile_n);
     const int M = i8_rows(A.n_rows, A.M);
     const int m0 = tile_m * BM, n0 = tile_n * BN;
     if (m0 >= M) return;
-    const int ks = blockIdx.y * A.k_split;
+    const int ks = split * A.k_split;
     const int ke = ks + A.k_split < A.K ? ks + A.k_split : A.K;
     const int rows_a = M - m0 < BM ? M - m0 : BM, rows_b = A.N - n0 < BN ? A.N - n0 : BN;
     const int kp = (A.K + 15) & ~15;
@@ -236,7 +236,7 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A)
             for (int tn = 0; tn < TN; ++tn) {
                 const int n = nw + tn * 16;
                 if (n >= A.N) continue;
-                const int64_t at = ((int64_t)blockIdx.y * A.M + m) * li_ld4(A.N) + n;
+                const int64_t at = ((int64_t)split * A.M + m) * li_ld4(A.N) + n;
                 if (P == 1) {
                     *(i32x4 *)((int32_t *)A.partial + at) = acc[0][tm][tn];
                 } else {
@@ -290,17 +290,26 @@ template <int BM, int BN, int WM, int WN, int P, int OCC>
 __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, OCC)
 linear_i8_kernel(const LiArgs A)
 {
-    linear_i8_tile<BM, BN, WM, WN, P>(A);
+    linear_i8_tile<BM, BN, WM, WN, P>(A, blockIdx.x, blockIdx.y);
+}
+
+// Both gradients' products in one launch: the first `blocks` workgroups are A's (tiles of a split next to each other), the
+// rest B's.
+template <int BM, int BN, int WM, int WN, int OCC>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, OCC)
+linear_i8_grad_kernel(const LiArgs A, const LiArgs B, int blocks)
+{
+    const bool second = (int)blockIdx.x >= blocks;
+    const LiArgs &R = second ? B : A;
+    const int i = second ? blockIdx.x - blocks : blockIdx.x, tiles = R.tiles_m * R.tiles_n;
+    linear_i8_tile<BM, BN, WM, WN, 3>(R, i % tiles, i / tiles);
 }
 // Joins the sums of a split k: a lane takes four neighbours.  (Letting the split that arrives last do this, behind a
 // device-scope fence, was tried: the fence writes back the whole L2 and the product of 2,000 x 12,544 x 1,024 went from 44
 // to 165 us.)
-template <int P>
-__global__ void __launch_bounds__(64)
-linear_i8_join_kernel(const LiArgs A)
+template <int P> __device__ __forceinline__ void linear_i8_join(const LiArgs &A, int64_t i)
 {
     const int quads = li_ld4(A.N) / 4;
-    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
     if (m >= i8_rows(A.n_rows, A.M)) return;
     const int64_t step = (int64_t)A.M * quads;
@@ -330,6 +339,17 @@ linear_i8_join_kernel(const LiArgs A)
     if (A.out_type == FRCNN_F32) li_store((float *)A.out + at, z, A.N - n);
     else if (A.out_type == FRCNN_BF16) li_store((__bf16 *)A.out + at, z, A.N - n);
     else li_store((_Float16 *)A.out + at, z, A.N - n);
+}
+
+__global__ void __launch_bounds__(64) linear_i8_join_kernel(const LiArgs A)
+{
+    linear_i8_join<1>(A, (int64_t)blockIdx.x * 64 + threadIdx.x);
+}
+
+__global__ void __launch_bounds__(64) linear_i8_grad_join_kernel(const LiArgs A, const LiArgs B, int blocks)
+{
+    const bool second = (int)blockIdx.x >= blocks;
+    linear_i8_join<3>(second ? B : A, (int64_t)(second ? blockIdx.x - blocks : blockIdx.x) * 64 + threadIdx.x);
 }
 
 // ---- a few rows -----------------------------------------------------------------------------------------------------
@@ -617,17 +637,15 @@ struct LiPlan {
     int64_t tiles;
 };
 
-// Tile by the rows there are; k is split until about every CU has a workgroup, down to eight stages each.
-static LiPlan li_plan(int M, int N, int K, int P)
+// k is split until about every CU has a workgroup, down to eight stages each.
+static LiPlan li_split(int bm, int bn, int M, int N, int K, int target)
 {
     LiPlan p;
-    p.bm = p.bn = 64;
-    if (P == 1 && M <= 32) p.bm = 32;
-    else if (P == 1 && (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) p.bm = p.bn = 256;
-    else if (M > 64 && N > 64) p.bm = p.bn = 128;
-    p.tiles = (int64_t)((M + p.bm - 1) / p.bm) * ((N + p.bn - 1) / p.bn);
+    p.bm = bm;
+    p.bn = bn;
+    p.tiles = (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     const int steps = (K + LI_BK - 1) / LI_BK;
-    int64_t want = p.tiles >= 256 ? 1 : 256 / p.tiles;
+    int64_t want = p.tiles >= 256 ? 1 : target / p.tiles;
     const int most = steps / 8 > 0 ? steps / 8 : 1;
     if (want > most) want = most;
     if (want < 1) want = 1;
@@ -637,35 +655,65 @@ static LiPlan li_plan(int M, int N, int K, int P)
     return p;
 }
 
-static size_t li_split_bytes(const LiPlan &p, int M, int N, int P)
+// Tile by the rows there are.
+static LiPlan li_plan(int M, int N, int K)
 {
-    return p.splits > 1 ? (size_t)p.splits * M * li_ld4(N) * (P == 3 ? 8 : 4) : 0;
+    int bm = 64, bn = 64;
+    if (M <= 32) bm = 32;
+    else if ((int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) bm = bn = 256;
+    else if (M > 64 && N > 64) bm = bn = 128;
+    return li_split(bm, bn, M, N, K, 256);
 }
 
-template <int P> static int li_launch(LiArgs &A, const LiPlan &p, void *split, hipStream_t st)
+// The gradients' tiles: of the same size for both products, so that one launch takes them.
+static LiPlan li_grad_plan(int rows, int cols, int inner) { return li_split(64, cols > 64 ? 128 : 64, rows, cols, inner, 256); }
+
+static size_t li_split_bytes(const LiPlan &p, int M, int N, int bytes)
+{
+    return p.splits > 1 ? up256((size_t)p.splits * M * li_ld4(N) * bytes) : 0;
+}
+
+static void li_apply(LiArgs &A, const LiPlan &p, void *split)
 {
     A.tiles_m = (A.M + p.bm - 1) / p.bm;
     A.tiles_n = (A.N + p.bn - 1) / p.bn;
     A.k_split = p.k_split;
     A.splits = p.splits;
     A.partial = split;
+}
+
+static int64_t li_join_blocks(const LiArgs &A) { return ((int64_t)A.M * (li_ld4(A.N) / 4) + 63) / 64; }
+
+static int li_launch(LiArgs &A, const LiPlan &p, void *split, hipStream_t st)
+{
+    li_apply(A, p, split);
     FRCNN_REQUIRE(p.tiles < (1ll << 31), "linear_i8: too many tiles");
     const dim3 grid((unsigned)p.tiles, p.splits);
-    if (p.bm == 256) {
-        hipLaunchKernelGGL((linear_i8_kernel<256, 256, 64, 128, 1, 2>), grid, dim3(512), 0, st, A);
-    } else if (p.bm == 128) {
-        if (P == 1) hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 64, 1, 2>), grid, dim3(256), 0, st, A);
-        else hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 32, 3, 2>), grid, dim3(512), 0, st, A);
-    } else if (p.bm == 64) {
-        hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, P, 1>), grid, dim3(256), 0, st, A);
-    } else {
-        hipLaunchKernelGGL((linear_i8_kernel<32, 64, 32, 32, 1, 1>), grid, dim3(128), 0, st, A);
-    }
+    if (p.bm == 256) hipLaunchKernelGGL((linear_i8_kernel<256, 256, 64, 128, 1, 2>), grid, dim3(512), 0, st, A);
+    else if (p.bm == 128) hipLaunchKernelGGL((linear_i8_kernel<128, 128, 64, 64, 1, 2>), grid, dim3(256), 0, st, A);
+    else if (p.bm == 64) hipLaunchKernelGGL((linear_i8_kernel<64, 64, 32, 32, 1, 1>), grid, dim3(256), 0, st, A);
+    else hipLaunchKernelGGL((linear_i8_kernel<32, 64, 32, 32, 1, 1>), grid, dim3(128), 0, st, A);
     FRCNN_CHECK_LAUNCH("linear_i8");
     if (p.splits > 1) {
-        const int64_t quads = (int64_t)A.M * (li_ld4(A.N) / 4);
-        hipLaunchKernelGGL((linear_i8_join_kernel<P>), dim3((unsigned)((quads + 63) / 64)), dim3(64), 0, st, A);
+        hipLaunchKernelGGL(linear_i8_join_kernel, dim3((unsigned)li_join_blocks(A)), dim3(64), 0, st, A);
         FRCNN_CHECK_LAUNCH("linear_i8_join");
+    }
+    return FRCNN_OK;
+}
+
+// A, and B where B.out is not NULL
+static int li_grad_launch(const LiArgs &A, const LiArgs &B, int bn, hipStream_t st)
+{
+    const int64_t a = A.out ? (int64_t)A.tiles_m * A.tiles_n * A.splits : 0, b = B.out ? (int64_t)B.tiles_m * B.tiles_n * B.splits : 0;
+    if (bn == 128)
+        hipLaunchKernelGGL((linear_i8_grad_kernel<64, 128, 32, 64, 2>), dim3((unsigned)(a + b)), dim3(256), 0, st, A, B, (int)a);
+    else
+        hipLaunchKernelGGL((linear_i8_grad_kernel<64, 64, 32, 32, 1>), dim3((unsigned)(a + b)), dim3(256), 0, st, A, B, (int)a);
+    FRCNN_CHECK_LAUNCH("linear_i8_grad");
+    const int64_t ja = A.out && A.splits > 1 ? li_join_blocks(A) : 0, jb = B.out && B.splits > 1 ? li_join_blocks(B) : 0;
+    if (ja + jb) {
+        hipLaunchKernelGGL(linear_i8_grad_join_kernel, dim3((unsigned)(ja + jb)), dim3(64), 0, st, A, B, (int)ja);
+        FRCNN_CHECK_LAUNCH("linear_i8_grad_join");
     }
     return FRCNN_OK;
 }
@@ -755,7 +803,7 @@ static LiArgs li_args(const int8_t *a, int64_t a_stride, const float *a_scale, c
 }
 
 // Workspace: [sums of a split k][codes of b on an aligned stride][codes of a on an aligned stride][a's scales]
-static size_t li_ws_b(int M, int N, int K) { return up256(li_split_bytes(li_plan(M, N, K, 1), M, N, 1)); }
+static size_t li_ws_b(int M, int N, int K) { return li_split_bytes(li_plan(M, N, K), M, N, 4); }
 static size_t li_ws_a(int M, int N, int K) { return li_ws_b(M, N, K) + up256((size_t)N * li_stride(K)); }
 static size_t li_ws_scale(int M, int N, int K) { return li_ws_a(M, N, K) + up256((size_t)M * li_stride(K)); }
 
@@ -782,11 +830,11 @@ extern "C" int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a
         frcnn_set_error("matmul_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
         return FRCNN_EWORKSPACE;
     }
-    const LiPlan p = li_plan(M, N, K, 1);
+    const LiPlan p = li_plan(M, N, K);
     char *ws = (char *)workspace;
     int rc = li_in_rows(&A.a, &A.a_stride, M, K, ws + li_ws_a(M, N, K), st);
     if (rc == FRCNN_OK) rc = li_in_rows(&A.b, &A.b_stride, N, K, ws + li_ws_b(M, N, K), st);
-    return rc == FRCNN_OK ? li_launch<1>(A, p, ws, st) : rc;
+    return rc == FRCNN_OK ? li_launch(A, p, ws, st) : rc;
 }
 
 extern "C" size_t frcnn_linear_i8_workspace_bytes(int M, int N, int K)
@@ -822,35 +870,94 @@ extern "C" int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, cons
         frcnn_set_error("linear_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
         return FRCNN_EWORKSPACE;
     }
-    const LiPlan p = li_plan(M, N, K, 1);
+    const LiPlan p = li_plan(M, N, K);
     char *ws = (char *)workspace;
     int8_t *codes = (int8_t *)(ws + li_ws_a(M, N, K));
     float *scale = (float *)(ws + li_ws_scale(M, N, K));
     A.a = codes;
     A.a_scale = scale;
-    int rc = frcnn_i8_quantize(x, x_type, x_stride, M, K, n_rows, codes, li_stride(K), scale, st);
+    int rc = frcnn_i8_quantize(I8Rows{x, x_type, x_stride, M, n_rows, codes, li_stride(K), scale}, I8Rows{}, K, st);
     if (rc == FRCNN_OK) rc = li_in_rows(&A.b, &A.b_stride, N, K, ws + li_ws_b(M, N, K), st);
-    return rc == FRCNN_OK ? li_launch<1>(A, p, ws, st) : rc;
+    return rc == FRCNN_OK ? li_launch(A, p, ws, st) : rc;
 }
 
-// Workspace of the gradients: for dL/dx the digits (3, M, N), their magnitudes, b transposed (K, N) and the sums of a
-// split; for dL/dw the digits (3, N, M), magnitudes, column partials, a transposed (K, M) and the sums of a split.
+// ---- training ----------------------------------------------------------------------------------------------------------
+// Codes and scales of both operands lie one behind the other in the caller's `saved`: a (M, ld), a_scale, b (N, ld), b_scale.
+struct LiSaved {
+    size_t a, a_scale, b, b_scale, total;
+};
+static LiSaved li_saved(int M, int N, int K)
+{
+    LiSaved s;
+    s.a = 0;
+    s.a_scale = s.a + up256((size_t)M * li_stride(K));
+    s.b = s.a_scale + up256((size_t)M * 4);
+    s.b_scale = s.b + up256((size_t)N * li_stride(K));
+    s.total = s.b_scale + up256((size_t)N * 4);
+    return s;
+}
+
+extern "C" size_t frcnn_linear_i8_train_saved_bytes(int M, int N, int K)
+{
+    return !li_shape_ok(M, N, K) || M == 0 ? 0 : li_saved(M, N, K).total;
+}
+
+extern "C" size_t frcnn_linear_i8_train_workspace_bytes(int M, int N, int K)
+{
+    return !li_shape_ok(M, N, K) || M == 0 || lf_takes(M, K) ? 0 : li_ws_b(M, N, K);
+}
+
+extern "C" int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride, const void *w, int w_type,
+                                     int64_t w_stride, const float *bias, int relu, int M, int N, int K, void *out,
+                                     int out_type, int64_t out_stride, void *saved, size_t saved_bytes, void *workspace,
+                                     size_t workspace_bytes, void *stream)
+{
+    FRCNN_REQUIRE(li_shape_ok(M, N, K) && M > 0, "linear_i8_train: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(i8_type_ok(x_type) && i8_type_ok(w_type) && i8_type_ok(out_type), "linear_i8_train: unknown element type");
+    FRCNN_REQUIRE(x_stride >= 0 && w_stride >= 0 && out_stride >= N, "linear_i8_train: bad strides");
+    FRCNN_REQUIRE(x && w && out, "linear_i8_train: null pointer");
+    const LiSaved l = li_saved(M, N, K);
+    const size_t need = frcnn_linear_i8_train_workspace_bytes(M, N, K);
+    if (!saved || saved_bytes < l.total || workspace_bytes < need || (need && !workspace)) {
+        frcnn_set_error("linear_i8_train: saved (%zu of %zu bytes) or workspace (%zu of %zu) too small", saved_bytes, l.total,
+                        workspace_bytes, need);
+        return FRCNN_EWORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t ld = li_stride(K);
+    char *s = (char *)saved;
+    const I8Rows a = {x, x_type, x_stride, M, nullptr, (int8_t *)(s + l.a), ld, (float *)(s + l.a_scale)};
+    const I8Rows b = {w, w_type, w_stride, N, nullptr, (int8_t *)(s + l.b), ld, (float *)(s + l.b_scale)};
+    const int rc = frcnn_i8_quantize(a, b, K, st);
+    if (rc != FRCNN_OK) return rc;
+    LiArgs A = li_args(a.codes, ld, a.scale, b.codes, ld, b.scale, bias, relu, M, N, K, nullptr, out, out_type, out_stride);
+    if (lf_takes(M, K)) return lf_launch(A, a.codes, ld, a.scale, st);
+    return li_launch(A, li_plan(M, N, K), workspace, st);
+}
+
+// Workspace of the gradients, part by part
 struct LiGrad {
-    size_t digits, top, partials, other, split, total;
-    LiPlan plan;
+    size_t x_split, x_digits, x_top, b_t, w_split, w_digits, w_top, a_t, part_top, part_sum, total;
+    LiPlan x, w;
 };
 
-static LiGrad li_grad_plan(int rows, int cols, int inner, size_t partials)
-{ // a product (rows, cols) over `inner`
+static LiGrad li_grad(int M, int N, int K)
+{
     LiGrad g;
-    const size_t ld = (size_t)li_stride(inner);
+    const size_t ldn = (size_t)li_stride(N), ldm = (size_t)li_stride(M), parts = (size_t)frcnn_i8_grad_parts(M) * N * 4;
     size_t off = 0;
-    g.plan = li_plan(rows, cols, inner, 3);
-    g.split = off; off += up256(li_split_bytes(g.plan, rows, cols, 3));
-    g.digits = off; off += up256(3 * (size_t)rows * ld);
-    g.top = off; off += up256((size_t)rows * 4);
-    g.partials = off; off += up256(partials);
-    g.other = off; off += up256((size_t)cols * ld);
+    g.x = li_grad_plan(M, K, N);
+    g.w = li_grad_plan(N, K, M);
+    g.x_split = off; off += li_split_bytes(g.x, M, K, 8);
+    g.x_digits = off; off += up256(3 * (size_t)M * ldn);
+    g.x_top = off; off += up256((size_t)M * 4);
+    g.b_t = off; off += up256((size_t)K * ldn);
+    g.w_split = off; off += li_split_bytes(g.w, N, K, 8);
+    g.w_digits = off; off += up256(3 * (size_t)N * ldm);
+    g.w_top = off; off += up256((size_t)N * 4);
+    g.a_t = off; off += up256((size_t)K * ldm);
+    g.part_top = off; off += up256(parts);
+    g.part_sum = off; off += up256(parts);
     g.total = off;
     return g;
 }
@@ -858,8 +965,7 @@ static LiGrad li_grad_plan(int rows, int cols, int inner, size_t partials)
 extern "C" size_t frcnn_linear_i8_backward_workspace_bytes(int M, int N, int K)
 {
     if (M <= 0 || N <= 0 || K <= 0 || M > I8_MAX_K || N > I8_MAX_K || K > I8_MAX_K) return 0;
-    const size_t x = li_grad_plan(M, K, N, 0).total, w = li_grad_plan(N, K, M, frcnn_i8_grad_col_partials(M, N)).total;
-    return x > w ? x : w;
+    return li_grad(M, N, K).total;
 }
 
 extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t grad_stride, const void *y,
@@ -874,37 +980,44 @@ extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t
                   "linear_i8_backward: unknown element type");
     FRCNN_REQUIRE(grad && a && a_scale && b && b_scale, "linear_i8_backward: null pointer");
     FRCNN_REQUIRE(grad_stride >= 0 && y_stride >= 0 && a_stride >= 0 && b_stride >= 0, "linear_i8_backward: bad strides");
-    const size_t need = frcnn_linear_i8_backward_workspace_bytes(M, N, K);
-    if (workspace_bytes < need || !workspace) {
-        frcnn_set_error("linear_i8_backward: workspace too small (%zu < %zu)", workspace_bytes, need);
+    const LiGrad l = li_grad(M, N, K);
+    if (workspace_bytes < l.total || !workspace) {
+        frcnn_set_error("linear_i8_backward: workspace too small (%zu < %zu)", workspace_bytes, l.total);
         return FRCNN_EWORKSPACE;
     }
+    if (!grad_x && !grad_w && !grad_bias) return FRCNN_OK;
     hipStream_t st = (hipStream_t)stream;
     char *ws = (char *)workspace;
-    int rc = FRCNN_OK;
+    const int64_t ldn = li_stride(N), ldm = li_stride(M);
+    I8Grad g = {};
+    g.grad = grad; g.type = grad_type; g.grad_stride = grad_stride;
+    g.y = y; g.y_stride = y_stride;
+    g.a = a; g.a_stride = a_stride; g.a_scale = a_scale;
+    g.b = b; g.b_stride = b_stride; g.b_scale = b_scale;
+    g.M = M; g.N = N; g.K = K;
+    g.row_stride = ldn; g.col_stride = ldm;
+    LiArgs X = {}, W = {};
     if (grad_x) {
-        const LiGrad g = li_grad_plan(M, K, N, 0);
-        const int64_t ld = li_stride(N), plane = (int64_t)M * ld;
-        LiArgs A = li_args((int8_t *)(ws + g.digits), ld, (float *)(ws + g.top), (int8_t *)(ws + g.other), ld, nullptr, nullptr,
-                           0, M, K, N, nullptr, grad_x, grad_x_type, K);
-        A.a_plane = plane;
-        rc = frcnn_i8_grad_row_digits(grad, grad_type, grad_stride, y, y_stride, b_scale, M, N, (int8_t *)(ws + g.digits), ld,
-                                      plane, (float *)(ws + g.top), st);
-        if (rc == FRCNN_OK) rc = frcnn_i8_transpose(b, b_stride, N, K, (int8_t *)(ws + g.other), ld, st);
-        if (rc == FRCNN_OK) rc = li_launch<3>(A, g.plan, ws + g.split, st);
-        if (rc != FRCNN_OK) return rc;
+        g.row_digits = (int8_t *)(ws + l.x_digits);
+        g.row_top = (float *)(ws + l.x_top);
+        g.b_t = (int8_t *)(ws + l.b_t);
+        X = li_args(g.row_digits, ldn, g.row_top, g.b_t, ldn, nullptr, nullptr, 0, M, K, N, nullptr, grad_x, grad_x_type, K);
+        X.a_plane = M * ldn;
+        li_apply(X, l.x, ws + l.x_split);
     }
     if (grad_w || grad_bias) { // the bias gradient is a by-product of the columns' magnitudes
-        const LiGrad g = li_grad_plan(N, K, M, frcnn_i8_grad_col_partials(M, N));
-        const int64_t ld = li_stride(M), plane = (int64_t)N * ld;
-        LiArgs A = li_args((int8_t *)(ws + g.digits), ld, (float *)(ws + g.top), (int8_t *)(ws + g.other), ld, nullptr, nullptr,
-                           0, N, K, M, nullptr, grad_w, grad_w_type, K);
-        A.a_plane = plane;
-        rc = frcnn_i8_grad_col_digits(grad, grad_type, grad_stride, y, y_stride, a_scale, M, N, (int8_t *)(ws + g.digits), ld,
-                                      plane, (float *)(ws + g.top), grad_bias, ws + g.partials, st);
-        if (!grad_w || rc != FRCNN_OK) return rc;
-        rc = frcnn_i8_transpose(a, a_stride, M, K, (int8_t *)(ws + g.other), ld, st);
-        if (rc == FRCNN_OK) rc = li_launch<3>(A, g.plan, ws + g.split, st);
+        g.col_digits = (int8_t *)(ws + l.w_digits);
+        g.col_top = (float *)(ws + l.w_top);
+        g.part_top = (uint32_t *)(ws + l.part_top);
+        g.part_sum = (float *)(ws + l.part_sum);
+        g.grad_bias = grad_bias;
     }
-    return rc;
+    if (grad_w) {
+        g.a_t = (int8_t *)(ws + l.a_t);
+        W = li_args(g.col_digits, ldm, g.col_top, g.a_t, ldm, nullptr, nullptr, 0, N, K, M, nullptr, grad_w, grad_w_type, K);
+        W.a_plane = N * ldm;
+        li_apply(W, l.w, ws + l.w_split);
+    }
+    const int rc = frcnn_i8_grad_prepare(g, st);
+    return rc != FRCNN_OK || (!grad_x && !grad_w) ? rc : li_grad_launch(X, W, l.x.bn, st);
 }

@@ -7,15 +7,16 @@
 // Two workgroups' rows have to fit a CU, so that one loads while the other computes: registers are bounded to 64.
 template <typename T, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS, 8)
-quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride, int M, int K, const int32_t *__restrict__ n_rows,
-                     int8_t *__restrict__ codes, int64_t c_stride, float *__restrict__ scale)
+quantize_rows_kernel(const I8Rows A, const I8Rows B, int K)
 {
     constexpr int V = 16 / sizeof(T);
     __shared__ uint32_t red[THREADS / 64];
-    const int row = blockIdx.x, t = threadIdx.x;
-    if (row >= i8_rows(n_rows, M)) return;
-    const T *xr = x + (int64_t)row * x_stride;
-    int8_t *cr = codes + (int64_t)row * c_stride;
+    const bool second = (int)blockIdx.x >= A.M;
+    const int row = second ? blockIdx.x - A.M : blockIdx.x, t = threadIdx.x;
+    if (!second && row >= i8_rows(A.n_rows, A.M)) return;
+    const T *xr = (const T *)(second ? B.x : A.x) + (int64_t)row * (second ? B.x_stride : A.x_stride);
+    const int64_t c_stride = second ? B.c_stride : A.c_stride;
+    int8_t *cr = (second ? B.codes : A.codes) + (int64_t)row * c_stride;
     const int kf = K - K % V; // whole vectors up to here; the last K % V elements one a thread
     I8Vec<T, V> v[NV];
     T v_tail = kf + t < K && t < V ? xr[kf + t] : (T)0.0f;
@@ -31,7 +32,7 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride, int M, int K, co
 #pragma unroll
         for (int j = 0; j < V; ++j) top_bits = qr_max(top_bits, qr_bits((float)v[i].v[j]));
     const QrRow q = qr_row(qr_block_max<THREADS>(top_bits, red));
-    if (t == 0) scale[row] = q.scale;
+    if (t == 0) (second ? B.scale : A.scale)[row] = q.scale;
     if (__builtin_expect(q.far, 0)) {
         v_tail = qr_lift(v_tail, q);
 #pragma unroll
@@ -63,34 +64,32 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t x_stride, int M, int K, co
 // Rows too long for the registers of a workgroup: the same in two passes over the row.
 template <typename T>
 __global__ void __launch_bounds__(1024)
-quantize_rows_long_kernel(const T *__restrict__ x, int64_t x_stride, int M, int K, const int32_t *__restrict__ n_rows,
-                          int8_t *__restrict__ codes, int64_t c_stride, float *__restrict__ scale)
+quantize_rows_long_kernel(const I8Rows A, int K)
 {
     __shared__ uint32_t red[16];
     const int row = blockIdx.x;
-    if (row >= i8_rows(n_rows, M)) return;
-    const T *xr = x + (int64_t)row * x_stride;
-    int8_t *cr = codes + (int64_t)row * c_stride;
+    if (row >= i8_rows(A.n_rows, A.M)) return;
+    const T *xr = (const T *)A.x + (int64_t)row * A.x_stride;
+    int8_t *cr = A.codes + (int64_t)row * A.c_stride;
     uint32_t top_bits = 0;
     for (int k = threadIdx.x; k < K; k += 1024) top_bits = qr_max(top_bits, qr_bits((float)xr[k]));
     const QrRow q = qr_row(qr_block_max<1024>(top_bits, red));
-    if (threadIdx.x == 0) scale[row] = q.scale;
-    const int end = (c_stride & 15) == 0 ? (K + 15) & ~15 : K;
+    if (threadIdx.x == 0) A.scale[row] = q.scale;
+    const int end = (A.c_stride & 15) == 0 ? (K + 15) & ~15 : K;
     for (int k = threadIdx.x; k < end; k += 1024)
         cr[k] = (int8_t)(q.none || k >= K ? 0 : qr_code((float)(q.far ? qr_lift(xr[k], q) : xr[k]), q));
 }
 
-template <typename T>
-static int quantize_rows_t(const T *x, int64_t x_stride, int M, int K, const int32_t *n_rows, int8_t *codes,
-                           int64_t c_stride, float *scale, hipStream_t st)
+// B: rows of a second matrix of the same type and length in the same launch (B.M = 0: none)
+template <typename T> static int quantize_rows_t(const I8Rows &A, const I8Rows &B, int K, hipStream_t st)
 {
     constexpr int V = 16 / sizeof(T);
-#define QR_LAUNCH(THREADS, NV)                                                                                      \
-    if (K <= THREADS * NV * V) {                                                                                    \
-        hipLaunchKernelGGL((quantize_rows_kernel<T, THREADS, NV>), dim3(M), dim3(THREADS), 0, st, x, x_stride, M, K, \
-                           n_rows, codes, c_stride, scale);                                                         \
-        FRCNN_CHECK_LAUNCH("quantize_rows");                                                                        \
-        return FRCNN_OK;                                                                                            \
+    const int M = A.M + B.M;
+#define QR_LAUNCH(THREADS, NV)                                                                            \
+    if (K <= THREADS * NV * V) {                                                                          \
+        hipLaunchKernelGGL((quantize_rows_kernel<T, THREADS, NV>), dim3(M), dim3(THREADS), 0, st, A, B, K); \
+        FRCNN_CHECK_LAUNCH("quantize_rows");                                                              \
+        return FRCNN_OK;                                                                                  \
     }
     // four loads a thread, or one where there are too few rows to fill the chip
     if (M >= 1024) {
@@ -107,20 +106,23 @@ static int quantize_rows_t(const T *x, int64_t x_stride, int M, int K, const int
         QR_LAUNCH(1024, 7) // what 64 registers hold
     }
 #undef QR_LAUNCH
-    hipLaunchKernelGGL((quantize_rows_long_kernel<T>), dim3(M), dim3(1024), 0, st, x, x_stride, M, K, n_rows, codes,
-                       c_stride, scale);
-    FRCNN_CHECK_LAUNCH("quantize_rows");
+    for (const I8Rows *r : {&A, &B}) {
+        if (r->M == 0) continue;
+        hipLaunchKernelGGL((quantize_rows_long_kernel<T>), dim3(r->M), dim3(1024), 0, st, *r, K);
+        FRCNN_CHECK_LAUNCH("quantize_rows");
+    }
     return FRCNN_OK;
 }
 
-int frcnn_i8_quantize(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows, int8_t *codes,
-                      int64_t codes_stride, float *scale, hipStream_t st)
+int frcnn_i8_quantize(const I8Rows &A, const I8Rows &B, int K, hipStream_t st)
 {
-    if (x_type == FRCNN_F32)
-        return quantize_rows_t((const float *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
-    if (x_type == FRCNN_BF16)
-        return quantize_rows_t((const __bf16 *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
-    return quantize_rows_t((const _Float16 *)x, x_stride, M, K, n_rows, codes, codes_stride, scale, st);
+    if (B.M && B.type != A.type) { // two types: two launches
+        const int rc = frcnn_i8_quantize(A, I8Rows{}, K, st);
+        return rc == FRCNN_OK ? frcnn_i8_quantize(B, I8Rows{}, K, st) : rc;
+    }
+    if (A.type == FRCNN_F32) return quantize_rows_t<float>(A, B, K, st);
+    if (A.type == FRCNN_BF16) return quantize_rows_t<__bf16>(A, B, K, st);
+    return quantize_rows_t<_Float16>(A, B, K, st);
 }
 
 extern "C" int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_stride, int M, int K, const int32_t *n_rows,
@@ -133,7 +135,8 @@ extern "C" int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_strid
     FRCNN_REQUIRE(x && codes && scale, "quantize_rows: null pointer");
     FRCNN_REQUIRE((codes_stride & 15) != 0 || ((uintptr_t)codes & 15) == 0,
                   "quantize_rows: codes of a padded row stride have to be 16-byte aligned");
-    return frcnn_i8_quantize(x, x_type, x_stride, M, K, n_rows, codes, codes_stride, scale, (hipStream_t)stream);
+    return frcnn_i8_quantize(I8Rows{x, x_type, x_stride, M, n_rows, codes, codes_stride, scale}, I8Rows{}, K,
+                             (hipStream_t)stream);
 }
 
 // ---- rows copied to an aligned row stride -----------------------------------------------------------------------
@@ -163,14 +166,23 @@ int frcnn_i8_pad_rows(const int8_t *src, int64_t src_stride, int rows, int K, in
     return FRCNN_OK;
 }
 
-// ---- byte transpose (rows, cols) -> (cols, rows): the operand of a gradient's product --------------------------------
-// 64 x 64 tiles through LDS; a thread reads 16 bytes of a row and writes 16 bytes of a column.
-__global__ void __launch_bounds__(256)
-i8_transpose_kernel(const int8_t *__restrict__ src, int64_t s_stride, int rows, int cols, int8_t *__restrict__ dst,
-                    int64_t d_stride)
+// ---- what the gradients' products are made from ----------------------------------------------------------------------
+// g_mn = grad_mn, or 0 where a ReLU's output y_mn is not above 0 (y = NULL: no ReLU; a NaN lets the gradient through, as
+// torch's threshold backward does).
+template <typename T> __device__ __forceinline__ float gd_grad(const T *grad, const T *y, int64_t gi, int64_t yi)
 {
-    __shared__ int8_t tile[64][68];
-    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
+    const float g = (float)grad[gi];
+    return y && (float)y[yi] <= 0.0f ? 0.0f : g;
+}
+
+// Fixed point relative to `top`: T = round(a I8_FIX / top), off by at most top 2^-24; the product and the factor are
+// formed in 64 bits.
+__device__ __forceinline__ int gd_fix(float a, double inv) { return (int)__builtin_rint((double)a * inv); }
+
+// Byte transpose (rows, cols) -> (cols, rows), one 64 x 64 tile; a thread reads 16 bytes of a row and writes 16 of a column.
+__device__ __forceinline__ void gd_transpose(const int8_t *src, int64_t s_stride, int rows, int cols, int8_t *dst,
+                                             int64_t d_stride, int64_t r0, int64_t c0, int8_t (&tile)[64][68])
+{
     const int tr = threadIdx.x >> 2, tc = (threadIdx.x & 3) * 16;
     uint32_t w[4] = {0, 0, 0, 0};
     if (r0 + tr < rows) {
@@ -191,51 +203,25 @@ i8_transpose_kernel(const int8_t *__restrict__ src, int64_t s_stride, int rows, 
     *(uint4 *)(dst + (c0 + tr) * d_stride + r0 + tc) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-int frcnn_i8_transpose(const int8_t *src, int64_t src_stride, int rows, int cols, int8_t *dst, int64_t dst_stride,
-                       hipStream_t stream)
-{
-    hipLaunchKernelGGL(i8_transpose_kernel, dim3((cols + 63) / 64, (rows + 63) / 64), dim3(256), 0, stream, src,
-                       src_stride, rows, cols, dst, dst_stride);
-    FRCNN_CHECK_LAUNCH("i8_transpose");
-    return FRCNN_OK;
-}
-
-// ---- digits of the gradients -----------------------------------------------------------------------------------------
-// g_mn = grad_mn, or 0 where a ReLU's output y_mn is not above 0 (y = NULL: no ReLU; a NaN lets the gradient through, as
-// torch's threshold backward does).
-template <typename T> __device__ __forceinline__ float gd_grad(const T *grad, const T *y, int64_t gi, int64_t yi)
-{
-    const float g = (float)grad[gi];
-    return y && (float)y[yi] <= 0.0f ? 0.0f : g;
-}
-
-// Fixed point relative to `top`: T = round(a I8_FIX / top), off by at most top 2^-24; the product and the factor are
-// formed in 64 bits.
-__device__ __forceinline__ int gd_fix(float a, double inv) { return (int)__builtin_rint((double)a * inv); }
-
-// For dL/dx: a_mn = g_mn * col_scale_n, fixed point relative to the row's largest magnitude.  One wave a row, four
+// For dL/dx: a_mn = g_mn * b_scale_n, fixed point relative to the row's largest magnitude.  One wave a row, four
 // neighbours a lane, up to NV of those held in registers; a longer row is read again (from the caches) for its digits.
 template <typename T, int NV>
-__global__ void __launch_bounds__(256)
-grad_row_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__restrict__ y, int64_t y_stride,
-                       const float *__restrict__ col_scale, int M, int N, int8_t *__restrict__ digits, int64_t stride,
-                       int64_t plane, float *__restrict__ row_top)
+__device__ __forceinline__ void gd_row_digits(const I8Grad &A, int64_t row)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= M) return;
-    const T *g = grad + row * g_stride, *z = y ? y + row * y_stride : nullptr;
+    const int lane = threadIdx.x & 63, N = A.N;
+    if (row >= A.M) return;
+    const T *g = (const T *)A.grad + row * A.grad_stride, *z = A.y ? (const T *)A.y + row * A.y_stride : nullptr;
     auto load = [&](float(&a)[4], int n) {
         if (n + 4 <= N) {
             const I8Vec<T, 4> v = i8_load<T, 4>(g + n);
-            const I8Vec<float, 4> c = i8_load<float, 4>(col_scale + n);
+            const I8Vec<float, 4> c = i8_load<float, 4>(A.b_scale + n);
             I8Vec<T, 4> u = v;
             if (z) u = i8_load<T, 4>(z + n);
 #pragma unroll
             for (int j = 0; j < 4; ++j) a[j] = (z && (float)u.v[j] <= 0.0f ? 0.0f : (float)v.v[j]) * c.v[j];
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] = n + j < N ? gd_grad(g, z, n + j, n + j) * col_scale[n + j] : 0.0f;
+            for (int j = 0; j < 4; ++j) a[j] = n + j < N ? gd_grad(g, z, n + j, n + j) * A.b_scale[n + j] : 0.0f;
         }
     };
     float a[NV][4];
@@ -256,8 +242,9 @@ grad_row_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
     const float top = __uint_as_float(top_bits);
     const bool none = !finite || top_bits == 0;
     const double inv = none ? 0.0 : (double)I8_FIX / (double)top;
-    if (lane == 0) row_top[row] = finite ? top : __builtin_nanf("");
-    int8_t *d = digits + row * stride;
+    if (lane == 0) A.row_top[row] = finite ? top : __builtin_nanf("");
+    int8_t *d = A.row_digits + row * A.row_stride;
+    const int64_t plane = A.M * A.row_stride;
     auto store = [&](const float(&t)[4], int n) {
         int q[3][4];
 #pragma unroll
@@ -267,51 +254,26 @@ grad_row_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if ((i * 64 + lane) * 4 < (int)stride) store(a[i], (i * 64 + lane) * 4);
-    for (int n = (NV * 64 + lane) * 4; n < (int)stride; n += 256) {
+        if ((i * 64 + lane) * 4 < (int)A.row_stride) store(a[i], (i * 64 + lane) * 4);
+    for (int n = (NV * 64 + lane) * 4; n < (int)A.row_stride; n += 256) {
         float t[4];
         load(t, n);
         store(t, n);
     }
 }
 
-int frcnn_i8_grad_row_digits(const void *grad, int type, int64_t grad_stride, const void *y, int64_t y_stride,
-                             const float *col_scale, int M, int N, int8_t *digits, int64_t stride, int64_t plane,
-                             float *row_top, hipStream_t stream)
-{
-#define GR_LAUNCH(T)                                                                                                    \
-    do {                                                                                                                \
-        if (N <= 256)                                                                                                   \
-            hipLaunchKernelGGL((grad_row_digits_kernel<T, 1>), dim3((M + 3) / 4), dim3(256), 0, stream, (const T *)grad, \
-                               grad_stride, (const T *)y, y_stride, col_scale, M, N, digits, stride, plane, row_top);   \
-        else                                                                                                            \
-            hipLaunchKernelGGL((grad_row_digits_kernel<T, 4>), dim3((M + 3) / 4), dim3(256), 0, stream, (const T *)grad, \
-                               grad_stride, (const T *)y, y_stride, col_scale, M, N, digits, stride, plane, row_top);   \
-    } while (0)
-    if (type == FRCNN_F32) GR_LAUNCH(float);
-    else if (type == FRCNN_BF16) GR_LAUNCH(__bf16);
-    else GR_LAUNCH(_Float16);
-#undef GR_LAUNCH
-    FRCNN_CHECK_LAUNCH("grad_row_digits");
-    return FRCNN_OK;
-}
-
-// For dL/dw: a_mn = g_mn * row_scale_m, fixed point relative to the COLUMN's largest magnitude, written transposed
-// (n, m).  First pass: largest magnitude and plain sum (dL/dbias) of every column over GC_ROWS rows; second pass: the
-// column's magnitude from those partials, the digits, and the sum of the partials in row order (the same bits every
+// For dL/dw: a_mn = g_mn * a_scale_m, fixed point relative to the COLUMN's largest magnitude, written transposed (n, m).
+// First the largest magnitude and the plain sum (dL/dbias) of every column over GC_ROWS rows; then (grad_col_digits_kernel)
+// the column's magnitude from those partials, the digits, and the sum of the partials in row order (the same bits every
 // run).
 #define GC_ROWS 64
 template <typename T>
-__global__ void __launch_bounds__(256)
-grad_col_partials_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__restrict__ y, int64_t y_stride,
-                         const float *__restrict__ row_scale, int M, int N, uint32_t *__restrict__ part_top,
-                         float *__restrict__ part_sum)
+__device__ __forceinline__ void gd_col_partials(const I8Grad &A, int bx, int by, uint32_t (&tops)[4][64], float (&sums)[4][64])
 {
-    __shared__ uint32_t tops[4][64];
-    __shared__ float sums[4][64];
+    const T *grad = (const T *)A.grad, *y = (const T *)A.y;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = blockIdx.x * 64 + lane;
-    const int64_t m0 = (int64_t)blockIdx.y * GC_ROWS;
+    const int n = bx * 64 + lane, N = A.N;
+    const int64_t m0 = (int64_t)by * GC_ROWS;
     uint32_t top = 0;
     float sum = 0.0f;
     if (n < N) {
@@ -319,8 +281,8 @@ grad_col_partials_kernel(const T *__restrict__ grad, int64_t g_stride, const T *
 #pragma unroll
         for (int i = 0; i < GC_ROWS / 4; ++i) {
             const int64_t m = m0 + i * 4 + wave;
-            g[i] = m < M ? gd_grad(grad, y, m * g_stride + n, m * y_stride + n) : 0.0f;
-            s[i] = m < M ? row_scale[m] : 0.0f;
+            g[i] = m < A.M ? gd_grad(grad, y, m * A.grad_stride + n, m * A.y_stride + n) : 0.0f;
+            s[i] = m < A.M ? A.a_scale[m] : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < GC_ROWS / 4; ++i) {
@@ -333,25 +295,52 @@ grad_col_partials_kernel(const T *__restrict__ grad, int64_t g_stride, const T *
     __syncthreads();
     if (wave == 0 && n < N) {
         for (int w = 1; w < 4; ++w) {
-            top = tops[w][lane] > top ? tops[w][lane] : top;
+            top = qr_max(top, tops[w][lane]);
             sum += sums[w][lane];
         }
-        part_top[(int64_t)blockIdx.y * N + n] = top;
-        part_sum[(int64_t)blockIdx.y * N + n] = sum;
+        A.part_top[(int64_t)by * N + n] = top;
+        A.part_sum[(int64_t)by * N + n] = sum;
+    }
+}
+
+// All that depends on nothing but the call's inputs, in one launch: workgroups [0, b0) row digits, [b0, b1) column
+// partials, [b1, b2) b transposed, [b2, b3) a transposed.
+template <typename T, int NV>
+__global__ void __launch_bounds__(256)
+grad_prepare_kernel(const I8Grad A, int b0, int b1, int b2)
+{
+    __shared__ union {
+        int8_t tile[64][68];
+        struct {
+            uint32_t tops[4][64];
+            float sums[4][64];
+        };
+    } s;
+    int b = blockIdx.x;
+    if (b < b0) {
+        gd_row_digits<T, NV>(A, (int64_t)b * 4 + (threadIdx.x >> 6));
+    } else if (b < b1) {
+        b -= b0;
+        const int nx = (A.N + 63) / 64;
+        gd_col_partials<T>(A, b % nx, b / nx, s.tops, s.sums);
+    } else {
+        const bool second = b >= b2;
+        b -= second ? b2 : b1;
+        const int nx = (A.K + 63) / 64;
+        if (second) gd_transpose(A.a, A.a_stride, A.M, A.K, A.a_t, A.col_stride, (int64_t)(b / nx) * 64, (int64_t)(b % nx) * 64, s.tile);
+        else gd_transpose(A.b, A.b_stride, A.N, A.K, A.b_t, A.row_stride, (int64_t)(b / nx) * 64, (int64_t)(b % nx) * 64, s.tile);
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-grad_col_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__restrict__ y, int64_t y_stride,
-                       const float *__restrict__ row_scale, int M, int N, int8_t *__restrict__ digits, int64_t stride,
-                       int64_t plane, float *__restrict__ col_top, float *__restrict__ col_sum,
-                       const uint32_t *__restrict__ part_top, const float *__restrict__ part_sum, int n_part)
+grad_col_digits_kernel(const I8Grad A, int n_part)
 {
     __shared__ int8_t tile[3][64][68]; // [digit][n][m]
     __shared__ double inv_s[64];
+    const T *grad = (const T *)A.grad, *y = (const T *)A.y;
     const int64_t m0 = (int64_t)blockIdx.y * 64;
-    const int n0 = blockIdx.x * 64;
+    const int n0 = blockIdx.x * 64, N = A.N;
     if (threadIdx.x < 64) {
         const int n = n0 + threadIdx.x;
         uint32_t top = 0;
@@ -359,15 +348,15 @@ grad_col_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
         if (n < N) {
 #pragma unroll 16
             for (int p = 0; p < n_part; ++p) {
-                top = qr_max(top, part_top[(int64_t)p * N + n]);
-                sum += part_sum[(int64_t)p * N + n];
+                top = qr_max(top, A.part_top[(int64_t)p * N + n]);
+                sum += A.part_sum[(int64_t)p * N + n];
             }
         }
         const bool finite = top < 0x7f800000u;
         inv_s[threadIdx.x] = !finite || top == 0 ? 0.0 : (double)I8_FIX / (double)__uint_as_float(top);
         if (blockIdx.y == 0 && n < N) {
-            col_top[n] = finite ? __uint_as_float(top) : __builtin_nanf("");
-            if (col_sum) col_sum[n] = sum;
+            A.col_top[n] = finite ? __uint_as_float(top) : __builtin_nanf("");
+            if (A.grad_bias) A.grad_bias[n] = sum;
         }
     }
     __syncthreads();
@@ -378,7 +367,7 @@ grad_col_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t m = m0 + wave * 16 + i;
-        a[i] = m < M && n < N ? gd_grad(grad, y, m * g_stride + n, m * y_stride + n) * row_scale[m] : 0.0f;
+        a[i] = m < A.M && n < N ? gd_grad(grad, y, m * A.grad_stride + n, m * A.y_stride + n) * A.a_scale[m] : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -391,36 +380,36 @@ grad_col_digits_kernel(const T *__restrict__ grad, int64_t g_stride, const T *__
     }
     __syncthreads();
     const int tn = threadIdx.x >> 2, tm = (threadIdx.x & 3) * 16;
-    if (n0 + tn >= N || m0 + tm >= stride) return;
+    if (n0 + tn >= N || m0 + tm >= A.col_stride) return;
     for (int p = 0; p < 3; ++p) {
         uint32_t w[4];
         for (int j = 0; j < 4; ++j) w[j] = *(const uint32_t *)&tile[p][tn][tm + 4 * j];
-        *(uint4 *)(digits + p * plane + (int64_t)(n0 + tn) * stride + m0 + tm) = make_uint4(w[0], w[1], w[2], w[3]);
+        *(uint4 *)(A.col_digits + ((int64_t)p * N + n0 + tn) * A.col_stride + m0 + tm) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
-size_t frcnn_i8_grad_col_partials(int M, int N)
+int frcnn_i8_grad_parts(int M) { return (M + GC_ROWS - 1) / GC_ROWS; }
+
+template <typename T> static int grad_prepare_t(const I8Grad &A, hipStream_t st)
 {
-    return (size_t)((M + GC_ROWS - 1) / GC_ROWS) * (size_t)N * 8;
+    const int nx = (A.N + 63) / 64, kx = (A.K + 63) / 64, mx = (A.M + 63) / 64, parts = frcnn_i8_grad_parts(A.M);
+    const int64_t b0 = A.row_digits ? (A.M + 3) / 4 : 0, b1 = b0 + (A.part_top ? (int64_t)nx * parts : 0),
+                  b2 = b1 + (A.b_t ? (int64_t)kx * nx : 0), b3 = b2 + (A.a_t ? (int64_t)kx * mx : 0);
+    if (A.N <= 256)
+        hipLaunchKernelGGL((grad_prepare_kernel<T, 1>), dim3((unsigned)b3), dim3(256), 0, st, A, (int)b0, (int)b1, (int)b2);
+    else
+        hipLaunchKernelGGL((grad_prepare_kernel<T, 4>), dim3((unsigned)b3), dim3(256), 0, st, A, (int)b0, (int)b1, (int)b2);
+    FRCNN_CHECK_LAUNCH("grad_prepare");
+    if (A.part_top) {
+        hipLaunchKernelGGL((grad_col_digits_kernel<T>), dim3(nx, mx), dim3(256), 0, st, A, parts);
+        FRCNN_CHECK_LAUNCH("grad_col_digits");
+    }
+    return FRCNN_OK;
 }
 
-int frcnn_i8_grad_col_digits(const void *grad, int type, int64_t grad_stride, const void *y, int64_t y_stride,
-                             const float *row_scale, int M, int N, int8_t *digits, int64_t stride, int64_t plane,
-                             float *col_top, float *col_sum, void *partials, hipStream_t stream)
+int frcnn_i8_grad_prepare(const I8Grad &A, hipStream_t st)
 {
-    const int n_part = (M + GC_ROWS - 1) / GC_ROWS;
-    uint32_t *part_top = (uint32_t *)partials;
-    float *part_sum = (float *)partials + (size_t)n_part * N;
-#define GC_LAUNCH(T)                                                                                                   \
-    hipLaunchKernelGGL((grad_col_partials_kernel<T>), dim3((N + 63) / 64, n_part), dim3(256), 0, stream, (const T *)grad, \
-                       grad_stride, (const T *)y, y_stride, row_scale, M, N, part_top, part_sum);                      \
-    hipLaunchKernelGGL((grad_col_digits_kernel<T>), dim3((N + 63) / 64, (M + 63) / 64), dim3(256), 0, stream,          \
-                       (const T *)grad, grad_stride, (const T *)y, y_stride, row_scale, M, N, digits, stride, plane,   \
-                       col_top, col_sum, part_top, part_sum, n_part)
-    if (type == FRCNN_F32) { GC_LAUNCH(float); }
-    else if (type == FRCNN_BF16) { GC_LAUNCH(__bf16); }
-    else { GC_LAUNCH(_Float16); }
-#undef GC_LAUNCH
-    FRCNN_CHECK_LAUNCH("grad_col_digits");
-    return FRCNN_OK;
+    if (A.type == FRCNN_F32) return grad_prepare_t<float>(A, st);
+    if (A.type == FRCNN_BF16) return grad_prepare_t<__bf16>(A, st);
+    return grad_prepare_t<_Float16>(A, st);
 }

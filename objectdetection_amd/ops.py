@@ -1148,19 +1148,35 @@ def linear_i8_backward(grad, y, codes, scale, weight_codes, weight_scale, x_dtyp
         return (torch.empty((0, K), dtype=x_dtype, device=dev) if want[0] else None,
                 torch.zeros((N, K), dtype=weight_dtype, device=dev) if want[1] else None,
                 torch.zeros((N,), dtype=torch.float32, device=dev) if want[2] else None)
-    grad, codes, weight_codes = _i8_codes(grad), _i8_codes(codes), _i8_codes(weight_codes)
-    y = _i8_codes(y) if y is not None else None
-    scale, weight_scale = _f32v(scale), _f32v(weight_scale)
+    codes, weight_codes, scale, weight_scale = _i8_codes(codes), _i8_codes(weight_codes), _f32v(scale), _f32v(weight_scale)
+    return _i8_backward(grad, y, codes.data_ptr(), _row_stride(codes), scale.data_ptr(), weight_codes.data_ptr(),
+                        _row_stride(weight_codes), weight_scale.data_ptr(), M, N, K, x_dtype, weight_dtype, want)
+
+
+def _i8_backward(grad, y, codes, codes_stride, scale, weight_codes, weight_stride, weight_scale, M, N, K, x_dtype,
+                 weight_dtype, want):
+    dev = grad.device
+    grad, y = _i8_codes(grad), (_i8_codes(y) if y is not None else None)
     gx = torch.empty((M, K), dtype=x_dtype, device=dev) if want[0] else None
     gw = torch.empty((N, K), dtype=weight_dtype, device=dev) if want[1] else None
     gb = torch.empty((N,), dtype=torch.float32, device=dev) if want[2] else None
     nbytes = _i8_workspace_bytes("frcnn_linear_i8_backward_workspace_bytes", M, N, K)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     _i8_call("frcnn_linear_i8_backward", dev, grad.data_ptr(), _I8_TYPES[grad.dtype], _row_stride(grad), _at(y),
-             _row_stride(y) if y is not None else 0, codes.data_ptr(), _row_stride(codes), scale.data_ptr(),
-             weight_codes.data_ptr(), _row_stride(weight_codes), weight_scale.data_ptr(), M, N, K, _at(gx),
-             _I8_TYPES[x_dtype], _at(gw), _I8_TYPES[weight_dtype], _at(gb), ws.data_ptr(), nbytes)
+             _row_stride(y) if y is not None else 0, codes, codes_stride, scale, weight_codes, weight_stride,
+             weight_scale, M, N, K, _at(gx), _I8_TYPES[x_dtype], _at(gw), _I8_TYPES[weight_dtype], _at(gb),
+             ws.data_ptr(), nbytes)
     return gx, gw, gb
+
+
+@functools.lru_cache(maxsize=1024)
+def _i8_saved(M, N, K):
+    """Offsets of what frcnn_linear_i8_train leaves for the backward call: x's scales, the weights' codes and scales."""
+    ld = (K + 15) // 16 * 16
+    up = lambda v: (v + 255) // 256 * 256  # noqa: E731
+    x_scale = up(M * ld)
+    w = x_scale + up(M * 4)
+    return ld, x_scale, w, w + up(N * ld)
 
 
 class LinearI8(torch.autograd.Function):
@@ -1176,20 +1192,48 @@ class LinearI8(torch.autograd.Function):
                              % (tuple(x.shape), tuple(weight.shape)))
         if x.dtype not in _I8_TYPES or weight.dtype not in _I8_TYPES:
             raise ValueError("LinearI8 takes float32, bfloat16 and float16; got %s, %s" % (x.dtype, weight.dtype))
-        codes, scale = quantize_rows_i8(x)
-        weight_codes, weight_scale = quantize_rows_i8(weight)
-        y = matmul_i8(codes, scale, weight_codes, weight_scale, bias, relu, x.dtype)
-        ctx.relu = bool(relu)
+        dev = x.device
+        _i8_device("LinearI8", dev, weight, bias)
+        M, K = x.shape
+        N = weight.shape[0]
+        if K == 0 or K > I8_MAX_K or N > I8_MAX_K or M > I8_MAX_K:
+            raise ValueError("LinearI8: (%d, %d, %d); each is at most %d and K at least 1" % (M, N, K, I8_MAX_K))
+        if bias is not None and bias.shape != (N,):
+            raise ValueError("LinearI8 expects a bias for each of the %d outputs; got %s" % (N, tuple(bias.shape)))
+        ctx.relu = relu = bool(relu)
         ctx.types = (x.dtype, weight.dtype, bias.dtype if bias is not None else None)
-        ctx.save_for_backward(codes, scale, weight_codes, weight_scale, *((y,) if relu else ()))
+        ctx.sizes = (M, N, K)
+        y = torch.empty((M, N), dtype=x.dtype, device=dev)
+        saved = torch.empty((_i8_workspace_bytes("frcnn_linear_i8_train_saved_bytes", M, N, K),), dtype=torch.uint8,
+                            device=dev)
+        if M > 0:
+            x, weight, bias = _i8_rows(x, "LinearI8"), _i8_rows(weight, "LinearI8"), _f32v(bias)
+            nbytes = _i8_workspace_bytes("frcnn_linear_i8_train_workspace_bytes", M, N, K)
+            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            _i8_call("frcnn_linear_i8_train", dev, x.data_ptr(), _I8_TYPES[x.dtype], _row_stride(x), weight.data_ptr(),
+                     _I8_TYPES[weight.dtype], _row_stride(weight), _at(bias), 1 if relu else 0, M, N, K, y.data_ptr(),
+                     _I8_TYPES[y.dtype], N, saved.data_ptr(), saved.numel(), ws.data_ptr(), nbytes)
+        if relu:
+            ctx.save_for_backward(saved, y)
+        else:
+            ctx.save_for_backward(saved)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         saved = ctx.saved_tensors
-        gx, gw, gb = linear_i8_backward(grad, saved[4] if ctx.relu else None, *saved[:4], ctx.types[0], ctx.types[1],
-                                        (tuple(ctx.needs_input_grad) + (False,))[:3])
-        if gb is not None and gb.dtype != ctx.types[2]:
-            gb = gb.to(ctx.types[2])
+        M, N, K = ctx.sizes
+        x_dtype, w_dtype, b_dtype = ctx.types
+        want = (tuple(ctx.needs_input_grad) + (False,))[:3]
+        if M == 0:
+            return (grad.new_empty((0, K), dtype=x_dtype) if want[0] else None,
+                    grad.new_zeros((N, K), dtype=w_dtype) if want[1] else None,
+                    grad.new_zeros((N,), dtype=b_dtype) if want[2] else None, None)
+        ld, x_scale, w, w_scale = _i8_saved(M, N, K)
+        at = saved[0].data_ptr()
+        gx, gw, gb = _i8_backward(grad, saved[1] if ctx.relu else None, at, ld, at + x_scale, at + w, ld, at + w_scale,
+                                  M, N, K, x_dtype, w_dtype, want)
+        if gb is not None and gb.dtype != b_dtype:
+            gb = gb.to(b_dtype)
         return gx, gw, gb, None
