@@ -655,13 +655,17 @@ static LiPlan li_split(int bm, int bn, int M, int N, int K, int target)
     return p;
 }
 
-// Tile by the rows there are.
+// A round of 256 x 256 tiles over the chip (256 of them, one a CU) takes five fourths of a round of 128 x 128 ones (512, two
+// a CU) and does twice as much; the small ones' last round counts by halves.  Rows of 6,272 by 1,024 channels, us, large :
+// medium tiles: 10,000 rows 77 : 95, 13,000 82 : 124, 18,000 162 : 158, 20,000 164 : 160, 24,000 162 : 190.  Up to 256 rows
+// 64 x 64 tiles, which need half as many splits (99 rows of 12,544 13.2 : 18.7, 300 19.4 : 18.6).
 static LiPlan li_plan(int M, int N, int K)
 {
+    const int64_t large = (int64_t)((M + 255) / 256) * ((N + 255) / 256), medium = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
     int bm = 64, bn = 64;
     if (M <= 32) bm = 32;
-    else if ((int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 256) bm = bn = 256;
-    else if (M > 64 && N > 64) bm = bn = 128;
+    else if ((large + 255) / 256 * 5 < (medium + 255) / 256 * 2) bm = bn = 256;
+    else if (M > 256 && N > 64) bm = bn = 128;
     return li_split(bm, bn, M, N, K, 256);
 }
 
