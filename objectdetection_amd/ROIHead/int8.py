@@ -1,0 +1,84 @@
+"""The box head's dense layers served in 8-bit integers (ops.linear_i8): the weights of a trained TwoMLPHead /
+FasterRCNNPredictor (ROIHead/mlp_head.py:19-49, ROIHead/predictor.py:19-49) quantised once, per output channel; the RoI
+features quantised per RoI on every call.  The reference runs these layers in fp32; no counterpart there.
+
+Drop-in for `mlp_head` / `predictor` of ROIHead, and for the padded path (`ROIPooling.forward_padded`): `n_rows`, the
+device-side row count, keeps the rows behind it out without a host read.  To train through the same rounding, construct
+the float modules with int8=True.
+"""
+import torch
+from torch.nn import Module
+
+from .. import ops
+
+
+class Int8Linear(Module):
+    """y = [relu](x W^T + b) with W as codes (N,K) int8 and scales (N) fp32.  Nothing here is trained: weights change only
+    by from_float or load_state_dict, and in training mode an x that wants a gradient is refused."""
+
+    def __init__(self, in_features, out_features, bias=True, relu=False):
+        super().__init__()
+        self.in_features, self.out_features, self.relu = in_features, out_features, relu
+        # rows on a stride of 16 bytes, which the kernels read in place
+        self.register_buffer("codes", torch.zeros((out_features, (in_features + 15) // 16 * 16), dtype=torch.int8))
+        self.register_buffer("scale", torch.zeros((out_features,)))
+        self.register_buffer("bias", torch.zeros((out_features,)) if bias else None)
+
+    @classmethod
+    def from_float(cls, weight, bias=None, relu=False):
+        """weight (N,K) and bias (N) or None, on a HIP device."""
+        layer = cls(weight.shape[1], weight.shape[0], bias is not None, relu).to(weight.device)
+        codes, scale = ops.quantize_rows_i8(weight.detach())
+        layer.codes[:, :weight.shape[1]] = codes
+        layer.scale.copy_(scale)
+        if bias is not None:
+            layer.bias.copy_(bias.detach())
+        return layer
+
+    def forward(self, x, n_rows=None, out_dtype=None):
+        if self.training and torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("Int8Linear has no gradient: call eval(), or train TwoMLPHead / FasterRCNNPredictor "
+                               "with int8=True")
+        return ops.linear_i8(x, self.codes[:, :self.in_features], self.scale, self.bias, self.relu, out_dtype, n_rows)
+
+
+class Int8TwoMLPHead(Module):
+    """TwoMLPHead served in 8-bit integers: flatten -> fc1 -> ReLU -> fc2 -> ReLU, the ReLUs inside the products."""
+
+    def __init__(self, in_channels, representation_size):
+        super().__init__()
+        self.fc1 = Int8Linear(in_channels, representation_size, relu=True)
+        self.fc2 = Int8Linear(representation_size, representation_size, relu=True)
+
+    @classmethod
+    def from_float(cls, head):
+        layer = cls.__new__(cls)
+        Module.__init__(layer)
+        layer.fc1 = Int8Linear.from_float(head.fc1.weight, head.fc1.bias, relu=True)
+        layer.fc2 = Int8Linear.from_float(head.fc2.weight, head.fc2.bias, relu=True)
+        return layer.train(head.training)
+
+    def forward(self, x, n_rows=None):
+        return self.fc2(self.fc1(x.flatten(start_dim=1), n_rows), n_rows)
+
+
+class Int8FasterRCNNPredictor(Module):
+    """FasterRCNNPredictor served in 8-bit integers: both of its layers in one product."""
+
+    def __init__(self, in_channels, num_classes):
+        super().__init__()
+        self.num_classes = num_classes
+        self.both = Int8Linear(in_channels, num_classes * 5)
+
+    @classmethod
+    def from_float(cls, predictor):
+        layer = cls.__new__(cls)
+        Module.__init__(layer)
+        layer.num_classes = predictor.cls_score.out_features
+        layer.both = Int8Linear.from_float(torch.cat([predictor.cls_score.weight, predictor.bbox_pred.weight]),
+                                           torch.cat([predictor.cls_score.bias, predictor.bbox_pred.bias]))
+        return layer.train(predictor.training)
+
+    def forward(self, x, n_rows=None):
+        y = self.both(x.flatten(start_dim=1), n_rows)
+        return y[:, :self.num_classes], y[:, self.num_classes:]

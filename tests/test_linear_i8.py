@@ -507,3 +507,155 @@ def test_other_stream_and_captured_replays(dev):
         got = [t.clone() for t in held]
         for u, v in zip(got, step()):
             same_bits(u, v)
+
+
+# ------------------------------------------------------------------------------------------------- the box head
+def _float_head(dev, in_channels=3 * 49, rep=70, classes=5, int8=False):
+    from objectdetection_amd.ROIHead import FasterRCNNPredictor, TwoMLPHead
+    torch.manual_seed(11)
+    return (TwoMLPHead(in_channels, rep, int8=int8).to(dev), FasterRCNNPredictor(rep, classes, int8=int8).to(dev))
+
+
+def _plain_layer(x, weight, bias, relu):
+    q, s = plain_codes(x)
+    p, t = plain_codes(weight)
+    return plain_product(q, s, p, t, bias.detach().cpu(), relu, F32)
+
+
+def _plain_head(x, head, pred):
+    """The served box head in 64 bits, layer by layer on the CPU."""
+    y = _plain_layer(x.flatten(1).cpu(), head.fc1.weight, head.fc1.bias, True)
+    y = _plain_layer(y, head.fc2.weight, head.fc2.bias, True)
+    return _plain_layer(y, pred.cls_score.weight, pred.cls_score.bias, False), \
+        _plain_layer(y, pred.bbox_pred.weight, pred.bbox_pred.bias, False)
+
+
+@gpu
+def test_served_box_head_behind_the_padded_pooling(dev):
+    """pool.forward_padded -> Int8TwoMLPHead -> Int8FasterRCNNPredictor with the device-side row count: the pooled rows
+    behind it hold NaN here, and the valid rows come out as from the unpadded features."""
+    from objectdetection_amd.ROIHead import Int8FasterRCNNPredictor, Int8TwoMLPHead, ROIPooling
+    head, pred = _float_head(dev)
+    served, served_pred = Int8TwoMLPHead.from_float(head).eval(), Int8FasterRCNNPredictor.from_float(pred).eval()
+    g = torch.Generator().manual_seed(3)
+    feat = torch.randn((2, 3, 20, 30), generator=g).relu().to(dev)
+    xy = torch.rand((2, 40, 2), generator=g) * 200
+    props = torch.cat([xy, xy + 20 + torch.rand((2, 40, 2), generator=g) * 100], 2).to(dev)
+    count = torch.tensor([40, 23], dtype=torch.int32, device=dev)
+    props[1, 23:] = 0
+    pool = ROIPooling(['1'], [7, 7], 2)
+    feats, total = pool.forward_padded({'1': feat}, props, count, [(320, 480)])
+    assert int(total) == 63
+    feats[63:] = float("nan")
+    cls, reg = served_pred(served(feats, total), total)
+    ref_cls, ref_reg = _plain_head(feats[:63], head, pred)
+    same_bits(cls[:63], ref_cls)
+    same_bits(reg[:63], ref_reg)
+    # and without a count, on the valid rows alone
+    cls, reg = served_pred(served(feats[:63]))
+    same_bits(cls, ref_cls)
+    same_bits(reg, ref_reg)
+
+
+@gpu
+def test_roi_head_serves_and_trains_through_int8(dev):
+    """ROIHead with the 8-bit layers: detections are those of the plain layers put in their place; its training branch
+    leaves the gradients that the chain of single calls gives, bit for bit, on the weights and on the feature maps."""
+    from objectdetection_amd import ops
+    from objectdetection_amd.ROIHead import Int8FasterRCNNPredictor, Int8TwoMLPHead, ROIHead, ROIPooling
+    g = torch.Generator().manual_seed(8)
+    xy = torch.rand((2, 60, 2), generator=g) * 150
+    boxes = torch.cat([xy, xy + 20 + torch.rand((2, 60, 2), generator=g) * 90], 2).to(dev)
+    props = [boxes[0], boxes[1, :35]]
+    targets = [{'size': [3.0, 281, 500], 'class': [1.0, 2.0], 'box': [[104, 78, 175, 183], [33, 88, 197, 123]]},
+               {'size': [3.0, 500.0, 375.0], 'class': [2.0], 'box': [[104, 78, 205, 183]]}]
+    head, pred = _float_head(dev)
+    with torch.no_grad():
+        pred.cls_score.weight.mul_(20)  # scores apart from each other
+    base = dict(pos_threshold=0.3, neg_threshold=0.3, num_sample=64, pos_fraction=0.25,
+                regression_weights=[10., 10., 5., 5.], score_thresh=0.05, proposal_min_size=1e-3, nms_threshold=0.5,
+                num_post_nms=50, roi_pooling=ROIPooling(['1', '2'], [7, 7], 2))
+    feats = [torch.randn((2, 3, 128, 128), generator=g).relu().to(dev), torch.randn((2, 3, 64, 64), generator=g).relu().to(dev)]
+
+    class Plain(torch.nn.Module):
+        def forward(self, x):
+            return x.flatten(1)
+
+    class PlainPredictor(torch.nn.Module):
+        def forward(self, x):
+            return tuple(t.to(dev) for t in _plain_head(x, head, pred))
+    args = (props, feats, (2, 256, 256), targets, [(250, 226), (256, 240)])
+    with torch.no_grad():
+        got, _ = ROIHead(dict(base, mlp_head=Int8TwoMLPHead.from_float(head),
+                              predictor=Int8FasterRCNNPredictor.from_float(pred)))(*args)
+        ref, _ = ROIHead(dict(base, mlp_head=Plain(), predictor=PlainPredictor()))(*args)
+    assert sum(len(r['score']) for r in ref) > 10
+    for a, b in zip(got, ref):
+        for key in ('proposal', 'score', 'label'):
+            assert torch.equal(a[key], b[key])
+
+    head, pred = _float_head(dev, int8=True)
+    maps = [f.clone().requires_grad_() for f in feats]
+    trained = ROIHead(dict(base, mlp_head=head, predictor=pred, force_eval=False)).train()
+    torch.manual_seed(4)
+    _, loss = trained(props, maps, (2, 256, 256), targets, [(250, 226), (256, 240)])
+    (loss["cls_loss"] + loss["reg_loss"]).backward()
+    # the same step by single calls
+    sampled = trained.last_sampled
+    again = [f.clone().requires_grad_() for f in feats]
+    pooled = trained.roi_pooling({'1': again[0], '2': again[1]}, [s["proposal"] for s in sampled], [(256, 256)])
+    x = pooled.flatten(1)
+    w3 = torch.cat([pred.cls_score.weight, pred.bbox_pred.weight]).detach()
+    b3 = torch.cat([pred.cls_score.bias, pred.bbox_pred.bias]).detach()
+    layers, y = [], x.detach()
+    for w, b, relu in ((head.fc1.weight, head.fc1.bias, True), (head.fc2.weight, head.fc2.bias, True), (w3, b3, False)):
+        c, s = ops.quantize_rows_i8(y)
+        p, t = ops.quantize_rows_i8(w)
+        y = ops.matmul_i8(c, s, p, t, b, relu)
+        layers.append((c, s, p, t, y if relu else None))
+    n = pred.cls_score.out_features
+    _, gl, gp = ops.roi_loss(y[:, :n], y[:, n:], torch.cat([s["cls_label"] for s in sampled]),
+                             torch.cat([s["reg_label"] for s in sampled]))
+    grad, grads = torch.cat([gl, gp.reshape(gl.shape[0], -1)], 1), []
+    for c, s, p, t, out in reversed(layers):
+        grad, gw, gb = ops.linear_i8_backward(grad, out, c, s, p, t)
+        grads.append((gw, gb))
+    same_bits(grads[2][0], head.fc1.weight.grad)
+    same_bits(grads[2][1], head.fc1.bias.grad)
+    same_bits(grads[1][0], head.fc2.weight.grad)
+    same_bits(grads[0][0], torch.cat([pred.cls_score.weight.grad, pred.bbox_pred.weight.grad]))
+    same_bits(grads[0][1], torch.cat([pred.cls_score.bias.grad, pred.bbox_pred.bias.grad]))
+    x.backward(grad)
+    for a, b in zip(maps, again):
+        # RoIAlign's backward adds with atomics for maps of this size: the order of its sums is not fixed
+        torch.testing.assert_close(a.grad, b.grad, rtol=1e-4, atol=1e-6 * float(b.grad.abs().max()))
+    assert head.fc1.weight.grad.abs().sum() > 0 and maps[0].grad.abs().sum() > 0
+
+
+@gpu
+def test_int8_modules_keep_and_refuse(dev):
+    from objectdetection_amd import _lib
+    from objectdetection_amd.ROIHead import Int8FasterRCNNPredictor, Int8Linear, Int8TwoMLPHead, TwoMLPHead
+    head, pred = _float_head(dev)
+    served = Int8TwoMLPHead.from_float(head)
+    other = Int8TwoMLPHead(3 * 49, 70).to(dev)
+    other.load_state_dict(served.state_dict())
+    x = features(9, 3 * 49, 2).to(dev)
+    same_bits(other(x), served(x))
+    assert set(served.state_dict()) == {"fc1.codes", "fc1.scale", "fc1.bias", "fc2.codes", "fc2.scale", "fc2.bias"}
+    assert not list(served.parameters())
+    loaded = Int8FasterRCNNPredictor(70, 5).to(dev)
+    loaded.load_state_dict(Int8FasterRCNNPredictor.from_float(pred).state_dict())
+    assert [t.shape for t in loaded(served(x))] == [(9, 5), (9, 20)]
+    bare = Int8Linear.from_float(head.fc2.weight)  # no bias, no ReLU, 16-bit output
+    y = bare(x[:, :70], out_dtype=BF16)
+    assert y.dtype == BF16 and (y < 0).any() and bare.bias is None
+    with pytest.raises(RuntimeError):
+        served.train()(x.requires_grad_())
+    served.eval()(x)  # serving: the result is detached
+    with torch.no_grad():
+        served.train()(x)
+    with pytest.raises(_lib.FrcnnError):
+        Int8TwoMLPHead.from_float(TwoMLPHead(8, 8))  # weights on the CPU
+    # same parameters, trained in 8 bits or not
+    assert set(TwoMLPHead(8, 8, int8=True).state_dict()) == set(TwoMLPHead(8, 8).state_dict())
