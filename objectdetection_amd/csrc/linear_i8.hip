@@ -6,6 +6,7 @@
 // matter, and splitting k over workgroups changes no bit.  The scales and the bias are applied in 64 bits and the
 // result is rounded to fp32 (and from there to 16 bits): the sign a ReLU looks at is the sign of the exact expression.
 #include "i8_common.h"
+#include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
@@ -23,6 +24,7 @@ struct LiArgs {
     int tiles_m, tiles_n, k_split;       // k_split: bytes of k per split, a multiple of LI_BK
     const float *a_scale, *b_scale, *bias;
     int relu, out_type;
+    bool stream;                         // results stored past the caches
     void *out;
     int64_t out_stride;                  // elements
     void *partial;                       // sums of a split k, (splits, M, li_ld4(N)) int32 (P = 3: int64), or NULL
@@ -47,18 +49,23 @@ template <int P> __device__ __forceinline__ double li_sum(int d0, int d1, int d2
     return P == 1 ? t : __builtin_fma(t, 65536.0, __builtin_fma((double)d1, 256.0, (double)d2));
 }
 
-// Four neighbours (the first `count` of them) in out's type; the address is aligned to one element.
-template <typename T> __device__ __forceinline__ void li_store(T *o, const float (&z)[4], int count)
+// V neighbours (the first `count` of them) in out's type; the address is aligned to one element.  STREAM: past the caches;
+// only where rows lie on 64 bytes, so that the 64 bytes which four lanes store are whole (pieces of 32 take twice as long).
+template <bool STREAM = false, typename T, int V> __device__ __forceinline__ void li_store(T *o, const float (&z)[V], int count)
 {
-    T h[4];
+    typedef int words __attribute__((ext_vector_type(V * sizeof(T) / 4), aligned(sizeof(T))));
+    T h[V];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) h[r] = (T)z[r];
-    if (count >= 4) {
-        __builtin_memcpy(o, h, sizeof(h));
+    for (int r = 0; r < V; ++r) h[r] = (T)z[r];
+    if (count >= V) {
+        words q;
+        __builtin_memcpy(&q, h, sizeof(h));
+        if constexpr (STREAM && sizeof(h) == 16) __builtin_nontemporal_store(q, (words *)o);
+        else *(words *)o = q;
     } else {
-        if (count > 0) o[0] = h[0];
-        if (count > 1) o[1] = h[1];
-        if (count > 2) o[2] = h[2];
+#pragma unroll
+        for (int r = 0; r < V - 1; ++r)
+            if (r < count) o[r] = h[r];
     }
 }
 
@@ -125,6 +132,9 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
                                                   (int)((rows_a - 1) * A.a_stride) + kp, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(A.b + (int64_t)n0 * A.b_stride), 0, (int)((rows_b - 1) * A.b_stride) + kp, 0x00020000);
+    // A lane's results of one 16 x 16 tile are four neighbours in n.  For 16-bit results the rows of b are dealt out so that
+    // those of two tiles make eight neighbours: 16 bytes a lane and 64 a row, as four of 32 bits are.
+    const bool pairs = TN % 2 == 0 && A.out_type != FRCNN_F32 && A.splits == 1;
     int va[GA], vb[GB];
     // rows of one wave's loads are RPL apart, a multiple of the swizzle's period or not: the chunk is per load
     int ca[GA], cb[GB];
@@ -138,7 +148,8 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
     for (int j = 0; j < GB; ++j) {
         const int r = (wave * GB + j) * RPL + lane / CPR;
         cb[j] = ((lane % CPR) ^ li_swz(r)) * 16;
-        vb[j] = r * (int)A.b_stride + cb[j];
+        const int n = pairs ? (r & ~31) + ((r >> 2) & 3) * 8 + ((r >> 4) & 1) * 4 + (r & 3) : r;
+        vb[j] = n * (int)A.b_stride + cb[j];
     }
     // Load i of a stage.  Chunks at and beyond the end of k are not read: their offset is beyond the buffer and the load
     // stores zeros.  A stage past the end is filled like any other, so that the loads in flight are the same in every step.
@@ -257,13 +268,14 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
         sa[tm] = mw + tm * 16 < M ? (double)A.a_scale[mw + tm * 16] : 0.0;
         if (P == 3) sa[tm] *= 1.0 / (double)I8_FIX;
     }
-    auto write = [&](auto *out) {
+    auto write = [&](auto *out, auto stream) {
+        constexpr int PT = sizeof(*out) == 2 && TN % 2 == 0 ? 2 : 1, V = 4 * PT; // tiles a store takes
 #pragma unroll
-        for (int tn = 0; tn < TN; ++tn) {
-            const int n = nw + tn * 16;
-            double sb[4], bias[4];
+        for (int tn = 0; tn < TN; tn += PT) {
+            const int n = n0 + wn0 + tn * 16 + q4 * V;
+            double sb[V], bias[V];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < V; ++r) {
                 const int nr = n + r < A.N ? n + r : A.N - 1;
                 sb[r] = P == 1 ? (double)A.b_scale[nr] : 1.0;
                 bias[r] = P == 1 && A.bias ? (double)A.bias[nr] : 0.0;
@@ -271,18 +283,24 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm) {
                 const int m = mw + tm * 16;
-                float z[4];
+                float z[V];
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    z[r] = li_finish(li_sum<P>(acc[0][tm][tn][r], acc[P > 1 ? 1 : 0][tm][tn][r], acc[P > 2 ? 2 : 0][tm][tn][r]),
+                for (int r = 0; r < V; ++r) {
+                    const int t = tn + r / 4, e = r % 4;
+                    z[r] = li_finish(li_sum<P>(acc[0][tm][t][e], acc[P > 1 ? 1 : 0][tm][t][e], acc[P > 2 ? 2 : 0][tm][t][e]),
                                      sa[tm], sb[r], bias[r], A.relu);
-                if (m < M) li_store(out + (int64_t)m * A.out_stride + n, z, A.N - n);
+                }
+                if (m < M) li_store<decltype(stream)::value>(out + (int64_t)m * A.out_stride + n, z, A.N - n);
             }
         }
     };
-    if (A.out_type == FRCNN_F32) write((float *)A.out);
-    else if (A.out_type == FRCNN_BF16) write((__bf16 *)A.out);
-    else write((_Float16 *)A.out);
+    auto write_as = [&](auto *out) { // (two copies: a choice at each store is merged into plain stores)
+        if (A.stream) write(out, std::true_type{});
+        else write(out, std::false_type{});
+    };
+    if (A.out_type == FRCNN_F32) write_as((float *)A.out);
+    else if (A.out_type == FRCNN_BF16) write_as((__bf16 *)A.out);
+    else write_as((_Float16 *)A.out);
 }
 
 // (The body is a device function: a kernel template with these builtins in it is dropped from the host pass.)
@@ -803,6 +821,7 @@ static LiArgs li_args(const int8_t *a, int64_t a_stride, const float *a_scale, c
     A.bias = bias; A.relu = relu;
     A.M = M; A.N = N; A.K = K; A.n_rows = n_rows;
     A.out = out; A.out_type = out_type; A.out_stride = out_stride;
+    A.stream = (((uintptr_t)out | (uint64_t)out_stride * i8_type_bytes(out_type)) & 63) == 0;
     return A;
 }
 
