@@ -338,30 +338,43 @@ grad_col_digits_kernel(const I8Grad A, int n_part)
 {
     __shared__ int8_t tile[3][64][68]; // [digit][n][m]
     __shared__ double inv_s[64];
+    __shared__ uint32_t tops[4][64];
+    __shared__ float sums[4][64];
     const T *grad = (const T *)A.grad, *y = (const T *)A.y;
     const int64_t m0 = (int64_t)blockIdx.y * 64;
     const int n0 = blockIdx.x * 64, N = A.N;
-    if (threadIdx.x < 64) {
-        const int n = n0 + threadIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = n0 + lane;
+    { // the column's magnitude and sum: a quarter of the partials a wave, the quarters in order
+        const int quarter = (n_part + 3) / 4, p0 = wave * quarter, p1 = p0 + quarter < n_part ? p0 + quarter : n_part;
         uint32_t top = 0;
         float sum = 0.0f;
         if (n < N) {
-#pragma unroll 16
-            for (int p = 0; p < n_part; ++p) {
+#pragma unroll 8
+            for (int p = p0; p < p1; ++p) {
                 top = qr_max(top, A.part_top[(int64_t)p * N + n]);
                 sum += A.part_sum[(int64_t)p * N + n];
             }
         }
+        tops[wave][lane] = top;
+        sums[wave][lane] = sum;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        uint32_t top = tops[0][lane];
+        float sum = sums[0][lane];
+        for (int w = 1; w < 4; ++w) {
+            top = qr_max(top, tops[w][lane]);
+            sum += sums[w][lane];
+        }
         const bool finite = top < 0x7f800000u;
-        inv_s[threadIdx.x] = !finite || top == 0 ? 0.0 : (double)I8_FIX / (double)__uint_as_float(top);
+        inv_s[lane] = !finite || top == 0 ? 0.0 : (double)I8_FIX / (double)__uint_as_float(top);
         if (blockIdx.y == 0 && n < N) {
             A.col_top[n] = finite ? __uint_as_float(top) : __builtin_nanf("");
             if (A.grad_bias) A.grad_bias[n] = sum;
         }
     }
     __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = n0 + lane;
     const double inv = inv_s[lane];
     float a[16]; // rows 16 wave .. 16 wave + 15 of the tile
 #pragma unroll

@@ -990,19 +990,29 @@ I8_MAX_K = 131071  # the 32-bit sums of the product cannot wrap up to here
 
 def _i8_call(name, dev, *args):
     """One entry point on dev's current stream."""
-    index = dev.index
+    index, fn = dev.index, getattr(_lib.load(), name)
     if torch.cuda.current_device() == index:
-        rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            rc = getattr(_lib.load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         _lib.check(rc, name)
 
 
 @functools.lru_cache(maxsize=1024)
-def _i8_workspace_bytes(name, M, N, K):
-    return max(getattr(_lib.load(), name)(M, N, K), 16)
+def _i8_bytes(name, M, N, K):
+    return getattr(_lib.load(), name)(M, N, K)
+
+
+def _i8_workspace(name, M, N, K, dev):
+    """-> (tensor or None, address or None, bytes): a fresh one for every call (the caching allocator ties it to the current
+    stream or graph), none where the call needs none."""
+    nbytes = _i8_bytes(name, M, N, K)
+    if nbytes == 0:
+        return None, None, 0
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr(), nbytes
 
 
 def _at(t):
@@ -1096,11 +1106,10 @@ def matmul_i8(codes, scale, weight_codes, weight_scale, bias=None, relu=False, o
     N, weight_codes, weight_scale, bias = _i8_weights(weight_codes, weight_scale, bias, K, dev, "matmul_i8")
     codes, scale, n_rows = _i8_codes(codes), _f32v(scale), _i8_count(n_rows, "matmul_i8", dev)
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    nbytes = _i8_workspace_bytes("frcnn_matmul_i8_workspace_bytes", M, N, K)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    ws, ws_at, nbytes = _i8_workspace("frcnn_matmul_i8_workspace_bytes", M, N, K, dev)
     _i8_call("frcnn_matmul_i8", dev, codes.data_ptr(), _row_stride(codes), scale.data_ptr(), weight_codes.data_ptr(),
              _row_stride(weight_codes), weight_scale.data_ptr(), _at(bias), 1 if relu else 0, M, N, K, _at(n_rows),
-             out.data_ptr(), _I8_TYPES[out_dtype], N, ws.data_ptr(), nbytes)
+             out.data_ptr(), _I8_TYPES[out_dtype], N, ws_at, nbytes)
     return out
 
 
@@ -1118,12 +1127,11 @@ def linear_i8(x, weight_codes, weight_scale, bias=None, relu=False, out_dtype=No
         raise ValueError("linear_i8: out_dtype is float32, bfloat16 or float16; got %s" % out_dtype)
     N, weight_codes, weight_scale, bias = _i8_weights(weight_codes, weight_scale, bias, K, dev, "linear_i8")
     n_rows = _i8_count(n_rows, "linear_i8", dev)
-    out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    nbytes = _i8_workspace_bytes("frcnn_linear_i8_workspace_bytes", M, N, K)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    out = x.new_empty((M, N), dtype=out_dtype)
+    ws, ws_at, nbytes = _i8_workspace("frcnn_linear_i8_workspace_bytes", M, N, K, dev)
     _i8_call("frcnn_linear_i8", dev, x.data_ptr(), _I8_TYPES[x.dtype], _row_stride(x), weight_codes.data_ptr(),
              _row_stride(weight_codes), weight_scale.data_ptr(), _at(bias), 1 if relu else 0, M, N, K, _at(n_rows),
-             out.data_ptr(), _I8_TYPES[out_dtype], N, ws.data_ptr(), nbytes)
+             out.data_ptr(), _I8_TYPES[out_dtype], N, ws_at, nbytes)
     return out
 
 
@@ -1160,12 +1168,11 @@ def _i8_backward(grad, y, codes, codes_stride, scale, weight_codes, weight_strid
     gx = torch.empty((M, K), dtype=x_dtype, device=dev) if want[0] else None
     gw = torch.empty((N, K), dtype=weight_dtype, device=dev) if want[1] else None
     gb = torch.empty((N,), dtype=torch.float32, device=dev) if want[2] else None
-    nbytes = _i8_workspace_bytes("frcnn_linear_i8_backward_workspace_bytes", M, N, K)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    ws, ws_at, nbytes = _i8_workspace("frcnn_linear_i8_backward_workspace_bytes", M, N, K, dev)
     _i8_call("frcnn_linear_i8_backward", dev, grad.data_ptr(), _I8_TYPES[grad.dtype], _row_stride(grad), _at(y),
              _row_stride(y) if y is not None else 0, codes, codes_stride, scale, weight_codes, weight_stride,
              weight_scale, M, N, K, _at(gx), _I8_TYPES[x_dtype], _at(gw), _I8_TYPES[weight_dtype], _at(gb),
-             ws.data_ptr(), nbytes)
+             ws_at, nbytes)
     return gx, gw, gb
 
 
@@ -1204,15 +1211,13 @@ class LinearI8(torch.autograd.Function):
         ctx.types = (x.dtype, weight.dtype, bias.dtype if bias is not None else None)
         ctx.sizes = (M, N, K)
         y = torch.empty((M, N), dtype=x.dtype, device=dev)
-        saved = torch.empty((_i8_workspace_bytes("frcnn_linear_i8_train_saved_bytes", M, N, K),), dtype=torch.uint8,
-                            device=dev)
+        saved = torch.empty((_i8_bytes("frcnn_linear_i8_train_saved_bytes", M, N, K),), dtype=torch.uint8, device=dev)
         if M > 0:
             x, weight, bias = _i8_rows(x, "LinearI8"), _i8_rows(weight, "LinearI8"), _f32v(bias)
-            nbytes = _i8_workspace_bytes("frcnn_linear_i8_train_workspace_bytes", M, N, K)
-            ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+            ws, ws_at, nbytes = _i8_workspace("frcnn_linear_i8_train_workspace_bytes", M, N, K, dev)
             _i8_call("frcnn_linear_i8_train", dev, x.data_ptr(), _I8_TYPES[x.dtype], _row_stride(x), weight.data_ptr(),
                      _I8_TYPES[weight.dtype], _row_stride(weight), _at(bias), 1 if relu else 0, M, N, K, y.data_ptr(),
-                     _I8_TYPES[y.dtype], N, saved.data_ptr(), saved.numel(), ws.data_ptr(), nbytes)
+                     _I8_TYPES[y.dtype], N, saved.data_ptr(), saved.numel(), ws_at, nbytes)
         if relu:
             ctx.save_for_backward(saved, y)
         else:
