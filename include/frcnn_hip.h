@@ -363,7 +363,7 @@ int frcnn_resize_pad_batch_f32(const float *const *src_host, const int32_t *shap
 /* ---- 8-bit dense layers of the box head ---------------------------------------------------------
  * The linear layers behind the RoI features (ROIHead/mlp_head.py:19-49, ROIHead/predictor.py:19-49; call site
  * ROIHead/roi_head.py:132-135) on 8-bit integers with one scale for every row (RoI) and one for every output
- * channel.  No counterpart in the reference, which runs them in fp32.
+ * channel.  No counterpart in the reference, which runs them in fp32.  At most 4,194,303 rows of any matrix.
  * Element types of `x`, `out` and the gradients: */
 #define FRCNN_F32 0
 #define FRCNN_BF16 1

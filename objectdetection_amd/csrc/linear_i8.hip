@@ -655,15 +655,14 @@ struct LiPlan {
     int64_t tiles;
 };
 
-// k is split until about every CU has a workgroup, down to eight stages each.
-static LiPlan li_split(int bm, int bn, int M, int N, int K, int target)
+// k in `want` parts, as many as come out even, down to eight stages each
+static LiPlan li_split(int bm, int bn, int M, int N, int K, int64_t want)
 {
     LiPlan p;
     p.bm = bm;
     p.bn = bn;
     p.tiles = (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     const int steps = (K + LI_BK - 1) / LI_BK;
-    int64_t want = p.tiles >= 256 ? 1 : target / p.tiles;
     const int most = steps / 8 > 0 ? steps / 8 : 1;
     if (want > most) want = most;
     if (want < 1) want = 1;
@@ -673,22 +672,47 @@ static LiPlan li_split(int bm, int bn, int M, int N, int K, int target)
     return p;
 }
 
-// A round of 256 x 256 tiles over the chip (256 of them, one a CU) takes five fourths of a round of 128 x 128 ones (512, two
-// a CU) and does twice as much; the small ones' last round counts by halves.  Rows of 6,272 by 1,024 channels, us, large :
-// medium tiles: 10,000 rows 77 : 95, 13,000 82 : 124, 18,000 162 : 158, 20,000 164 : 160, 24,000 162 : 190.  Up to 256 rows
-// 64 x 64 tiles, which need half as many splits (99 rows of 12,544 13.2 : 18.7, 300 19.4 : 18.6).
+// Up to 256 rows: 64 x 64 tiles (32 x 64 up to 32 rows), k split over the CUs; they need half as many splits as larger ones
+// (99 rows of 12,544 13.2 us : 18.7).  Above, 128 x 128 or 256 x 256 by an estimate of the time, in ns:
+//   256 x 256, one workgroup a CU: 870 a stage with the whole chip at it (there the clock gives way: 2.3 POPS), 700 at least;
+//   128 x 128: 320 a stage for each workgroup of a CU (1.6 POPS);
+//   and for a split k the sums' way out and back, at 8 TB/s, and a launch.
+// us, 256 : 128, by 1,024 channels: 2,000 rows of 12,544 49 : 44, 4,000 70 : 66, 6,000 90 : 113; of 25,088 2,048 rows 67 : 75,
+// 4,000 102 : 123, 6,000 146 : 233; of 6,272 13,000 rows 82 : 124, 20,000 164 : 160; 32,000 rows of 1,024 (to 16 bits) 45 : 61.
 static LiPlan li_plan(int M, int N, int K)
 {
-    const int64_t large = (int64_t)((M + 255) / 256) * ((N + 255) / 256), medium = (int64_t)((M + 127) / 128) * ((N + 127) / 128);
-    int bm = 64, bn = 64;
-    if (M <= 32) bm = 32;
-    else if ((large + 255) / 256 * 5 < (medium + 255) / 256 * 2) bm = bn = 256;
-    else if (M > 256 && N > 64) bm = bn = 128;
-    return li_split(bm, bn, M, N, K, 256);
+    if (M <= 256 || N <= 64) {
+        const int bm = M <= 32 ? 32 : 64;
+        const int64_t tiles = (int64_t)((M + bm - 1) / bm) * ((N + 63) / 64);
+        return li_split(bm, 64, M, N, K, 256 / tiles);
+    }
+    LiPlan best = {};
+    double least = 0.0;
+    for (int side = 128; side <= 256; side *= 2) {
+        const int64_t tiles = (int64_t)((M + side - 1) / side) * ((N + side - 1) / side);
+        for (int64_t want = 256 / tiles > 1 ? 256 / tiles : 1; want; want = want > 1 ? 1 : 0) {
+            const LiPlan p = li_split(side, side, M, N, K, want);
+            const int64_t blocks = tiles * p.splits, rounds = (blocks + 255) / 256;
+            const double stages = (double)(p.k_split / LI_BK), share = rounds > 1 ? 1.0 : (double)blocks / 256.0;
+            double ns = side == 256 ? rounds * (stages * (share * 870.0 > 700.0 ? share * 870.0 : 700.0) + 7000.0)
+                                    : rounds * stages * 320.0 + 5000.0;
+            if (p.splits > 1) ns += 4000.0 + (2.0 * p.splits + 1.0) * M * N * 4.0 / 8000.0;
+            if (best.splits == 0 || ns < least) {
+                best = p;
+                least = ns;
+            }
+        }
+    }
+    return best;
 }
 
 // The gradients' tiles: of the same size for both products, so that one launch takes them.
-static LiPlan li_grad_plan(int rows, int cols, int inner) { return li_split(64, cols > 64 ? 128 : 64, rows, cols, inner, 256); }
+static LiPlan li_grad_plan(int rows, int cols, int inner)
+{
+    const int bn = cols > 64 ? 128 : 64;
+    const int64_t tiles = (int64_t)((rows + 63) / 64) * ((cols + bn - 1) / bn);
+    return li_split(64, bn, rows, cols, inner, 256 / tiles);
+}
 
 static size_t li_split_bytes(const LiPlan &p, int M, int N, int bytes)
 {
@@ -750,7 +774,11 @@ static bool li_in_place(const void *p, int64_t stride, int K)
     return ((uintptr_t)p & 15) == 0 && (stride & 15) == 0 && stride >= K && stride <= LI_MAX_STRIDE;
 }
 
-static bool li_shape_ok(int M, int N, int K) { return M >= 0 && N > 0 && K > 0 && K <= I8_MAX_K && (int64_t)M * N < (1ll << 40); }
+static bool li_shape_ok(int M, int N, int K)
+{
+    return M >= 0 && M <= I8_MAX_ROWS && N > 0 && N <= I8_MAX_ROWS && K > 0 && K <= I8_MAX_K;
+}
+static bool li_ws_ok(const void *ws) { return ((uintptr_t)ws & 255) == 0; }
 
 // The few-rows form.  1,024 channels, rows of 12,544: 1 / 2 / 3 / 4 rows 5.5 / 8.6 / 11.9 / 15.2 us against 14.5 by tiles and
 // three launches, which cost the host 6 us more than one.
@@ -840,7 +868,8 @@ extern "C" int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a
                                const int32_t *n_rows, void *out, int out_type, int64_t out_stride, void *workspace,
                                size_t workspace_bytes, void *stream)
 {
-    FRCNN_REQUIRE(li_shape_ok(M, N, K), "matmul_i8: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(li_shape_ok(M, N, K), "matmul_i8: bad shape (%d, %d, %d); K is at most %d, M and N %d", M, N, K,
+                  I8_MAX_K, I8_MAX_ROWS);
     FRCNN_REQUIRE(i8_type_ok(out_type), "matmul_i8: unknown element type %d", out_type);
     FRCNN_REQUIRE(a_stride >= 0 && b_stride >= 0 && out_stride >= N, "matmul_i8: bad strides");
     if (M == 0) return FRCNN_OK;
@@ -849,6 +878,7 @@ extern "C" int frcnn_matmul_i8(const int8_t *a, int64_t a_stride, const float *a
     LiArgs A = li_args(a, a_stride, a_scale, b, b_stride, b_scale, bias, relu, M, N, K, n_rows, out, out_type, out_stride);
     if (lf_takes(M, K)) return lf_launch(A, a, a_stride, a_scale, st);
     const size_t need = li_ws_scale(M, N, K);
+    FRCNN_REQUIRE(li_ws_ok(workspace), "matmul_i8: the workspace has to be 256-byte aligned");
     if (workspace_bytes < need || !workspace) {
         frcnn_set_error("matmul_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
         return FRCNN_EWORKSPACE;
@@ -870,7 +900,8 @@ extern "C" int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, cons
                                const int32_t *n_rows, void *out, int out_type, int64_t out_stride, void *workspace,
                                size_t workspace_bytes, void *stream)
 {
-    FRCNN_REQUIRE(li_shape_ok(M, N, K), "linear_i8: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(li_shape_ok(M, N, K), "linear_i8: bad shape (%d, %d, %d); K is at most %d, M and N %d", M, N, K,
+                  I8_MAX_K, I8_MAX_ROWS);
     FRCNN_REQUIRE(i8_type_ok(x_type) && i8_type_ok(out_type), "linear_i8: unknown element type");
     FRCNN_REQUIRE(x_stride >= 0 && b_stride >= 0 && out_stride >= N, "linear_i8: bad strides");
     if (M == 0) return FRCNN_OK;
@@ -889,6 +920,7 @@ extern "C" int frcnn_linear_i8(const void *x, int x_type, int64_t x_stride, cons
         return lf_launch(A, (const _Float16 *)x, x_stride, nullptr, st);
     }
     const size_t need = frcnn_linear_i8_workspace_bytes(M, N, K);
+    FRCNN_REQUIRE(li_ws_ok(workspace), "linear_i8: the workspace has to be 256-byte aligned");
     if (workspace_bytes < need || !workspace) {
         frcnn_set_error("linear_i8: workspace too small (%zu < %zu)", workspace_bytes, need);
         return FRCNN_EWORKSPACE;
@@ -935,12 +967,15 @@ extern "C" int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride
                                      int out_type, int64_t out_stride, void *saved, size_t saved_bytes, void *workspace,
                                      size_t workspace_bytes, void *stream)
 {
-    FRCNN_REQUIRE(li_shape_ok(M, N, K) && M > 0, "linear_i8_train: bad shape (%d, %d, %d); K is at most %d", M, N, K, I8_MAX_K);
+    FRCNN_REQUIRE(li_shape_ok(M, N, K) && M > 0, "linear_i8_train: bad shape (%d, %d, %d); K is at most %d, M and N %d", M, N, K,
+                  I8_MAX_K, I8_MAX_ROWS);
     FRCNN_REQUIRE(i8_type_ok(x_type) && i8_type_ok(w_type) && i8_type_ok(out_type), "linear_i8_train: unknown element type");
     FRCNN_REQUIRE(x_stride >= 0 && w_stride >= 0 && out_stride >= N, "linear_i8_train: bad strides");
     FRCNN_REQUIRE(x && w && out, "linear_i8_train: null pointer");
     const LiSaved l = li_saved(M, N, K);
     const size_t need = frcnn_linear_i8_train_workspace_bytes(M, N, K);
+    FRCNN_REQUIRE(li_ws_ok(workspace) && li_ws_ok(saved), "linear_i8_train: saved and workspace have to be 256-byte aligned");
+    FRCNN_REQUIRE(M + N <= I8_MAX_ROWS, "linear_i8_train: M + N (%d) is at most %d", M + N, I8_MAX_ROWS);
     if (!saved || saved_bytes < l.total || workspace_bytes < need || (need && !workspace)) {
         frcnn_set_error("linear_i8_train: saved (%zu of %zu bytes) or workspace (%zu of %zu) too small", saved_bytes, l.total,
                         workspace_bytes, need);
@@ -1004,6 +1039,7 @@ extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t
     FRCNN_REQUIRE(grad && a && a_scale && b && b_scale, "linear_i8_backward: null pointer");
     FRCNN_REQUIRE(grad_stride >= 0 && y_stride >= 0 && a_stride >= 0 && b_stride >= 0, "linear_i8_backward: bad strides");
     const LiGrad l = li_grad(M, N, K);
+    FRCNN_REQUIRE(li_ws_ok(workspace), "linear_i8_backward: the workspace has to be 256-byte aligned");
     if (workspace_bytes < l.total || !workspace) {
         frcnn_set_error("linear_i8_backward: workspace too small (%zu < %zu)", workspace_bytes, l.total);
         return FRCNN_EWORKSPACE;

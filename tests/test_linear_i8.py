@@ -108,6 +108,19 @@ def test_c_entries_refuse_before_any_launch():
     refused(mm(t=9), b"element type")
     refused(mm(m=40, nb=16), b"workspace", -2)
     refused(mm(m=40, ws=null), b"workspace", -2)
+    refused(mm(m=40, ws=ctypes.c_void_p(4096 + 128)), b"aligned")
+    refused(mm(m=1 << 22), b"shape")
+    refused(lib.frcnn_quantize_rows_i8(p, 0, 8, 1 << 22, 8, null, p, 16, p, null), b"rows")
+
+    def tr(m=40, n=4, k=32, sv=p, sb=1 << 30, wb=1 << 30, x=p):
+        return lib.frcnn_linear_i8_train(x, 0, k, p, 0, k, null, 0, m, n, k, p, 0, n, sv, sb, p, wb, null)
+    refused(tr(m=0), b"shape")
+    refused(tr(k=131072), b"at most 131071")
+    refused(tr(x=null), b"null")
+    refused(tr(sb=16), b"saved", -2)
+    refused(tr(sv=null), b"saved", -2)
+    refused(tr(sv=ctypes.c_void_p(4096 + 64)), b"aligned")
+    refused(tr(m=4194303), b"M + N")
     refused(lib.frcnn_linear_i8(p, 0, 2048, p, 2048, p, null, 0, 40, 4, 2048, null, p, 0, 4, p, 16, null), b"workspace", -2)
     refused(lib.frcnn_linear_i8(null, 0, 32, p, 32, p, null, 0, 4, 4, 32, null, p, 0, 4, p, 16, null), b"null")
     refused(lib.frcnn_linear_i8(p, 0, 32, p, 32, p, null, 0, 4, 4, 32, null, p, 0, 3, p, 16, null), b"strides")
