@@ -785,12 +785,13 @@ static bool li_ws_ok(const void *ws) { return ((uintptr_t)ws & 255) == 0; }
 static bool lf_takes(int M, int K) { return M <= 4 && K <= LF_THREADS * LF_CHUNKS * 16; }
 
 // The short-rows form (K >= 16: the last weight is read by a 16-byte load).  It reads the weights once per BM rows, so it
-// gives way to quantiser and tiles where rows and channels are both many: rows of 1,024, us against us, at 105 channels
-// 8.9 : 11.2 (500 rows), 9.2 : 13.8 (2,000), 36 : 42 (32,000); at 256 9.6 : 12.3, 10.6 : 16.5, 45 : 48; at 1,024 10.4 : 15.0,
-// 20.2 : 24.5, 102 : 97 (and 4,000 rows 31 : 23).
+// gives way to quantiser and tiles where rows and channels are both many.  us against us, on the GPU (a call of three launches
+// also costs the host 6 us more): rows of 1,024 by 105 channels 8.9 : 11.2 (500 rows), 9.2 : 13.8 (2,000), 36.6 : 40.7
+// (32,000); by 256 10.6 : 16.5 (2,000), 24.6 : 21.7 (8,000); by 1,024 10.4 : 15.0 (500), 15.4 : 15.6 (1,000), 19.3 : 17.1
+// (2,000); 32,000 rows of 512 by 256 27.4 : 29.8.
 static bool lr_takes(int M, int N, int K)
 {
-    return K <= LR_K && K >= 16 && M > 2 && (N <= 256 || (int64_t)M * N <= (1 << 21));
+    return K <= LR_K && K >= 16 && M > 2 && (N <= 128 || (N <= 256 && K <= 512) || (int64_t)M * N <= (1 << 20));
 }
 
 template <typename T>

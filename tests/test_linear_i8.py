@@ -274,6 +274,24 @@ def test_matmul_i8(dev, m, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(13001, 771, 1153), (16300, 1000, 1000), (511, 505, 130001)])
+def test_matmul_i8_large_tiles(dev, m, n, k):
+    """Sizes that go by 256 x 256 tiles, the last with k split over the chip; rows behind a device-side count."""
+    from objectdetection_amd import ops
+    g = torch.Generator().manual_seed(k)
+    a = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8)
+    sa, sb, bias = torch.rand((m,), generator=g) * 0.1, torch.rand((n,), generator=g) * 0.01, torch.randn((n,), generator=g)
+    rows = torch.cat([torch.arange(0, m, max(1, m // 300)), torch.tensor([m - 1])])
+    ad, bd, sad, sbd, biasd = (t.to(dev) for t in (a, b, sa, sb, bias))
+    for out_dtype, relu, count in [(F32, True, None), (BF16, False, None), (F16, True, m - 130), (F32, False, 257)]:
+        cnt = torch.tensor([count], dtype=torch.int32, device=dev) if count else None
+        out = ops.matmul_i8(ad, sad, bd, sbd, biasd, relu, out_dtype, cnt).cpu()
+        at = rows[rows < (count or m)]
+        same_bits(out[at], plain_product(a[at], sa[at], b, sb, bias, relu, out_dtype))
+
+
+@gpu
 def test_matmul_i8_views(dev):
     """Rows of any stride and alignment give what contiguous rows give; what lies between them is not read into it."""
     from objectdetection_amd import ops
