@@ -35,6 +35,17 @@ class Int8Linear(Module):
             layer.bias.copy_(bias.detach())
         return layer
 
+    def _apply(self, fn, *args, **kwargs):
+        """half(), to(torch.bfloat16) and the like move the buffers but leave the scales and the bias in fp32: a weight's
+        scale in fp16 would be a subnormal number."""
+        kept = {"scale": self.scale, "bias": self.bias}
+        super()._apply(fn, *args, **kwargs)
+        for name, t in kept.items():
+            now = getattr(self, name)
+            if now is not None and now.dtype != t.dtype:
+                setattr(self, name, t.to(now.device))
+        return self
+
     def forward(self, x, n_rows=None, out_dtype=None):
         if self.training and torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("Int8Linear has no gradient: call eval(), or train TwoMLPHead / FasterRCNNPredictor "

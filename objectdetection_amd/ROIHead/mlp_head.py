@@ -6,6 +6,8 @@ from .. import ops
 
 
 class TwoMLPHead(Module):
+    int8 = False  # for modules pickled whole before there was a choice
+
     def __init__(self, in_channels, representation_size, int8=False):
         super().__init__()
         self.fc1 = Linear(in_channels, representation_size)

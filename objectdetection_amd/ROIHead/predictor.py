@@ -8,6 +8,8 @@ from .. import ops
 
 
 class FasterRCNNPredictor(Module):
+    int8 = False  # for modules pickled whole before there was a choice
+
     def __init__(self, in_channels, num_classes, int8=False):
         super().__init__()
         self.cls_score = Linear(in_channels, num_classes)

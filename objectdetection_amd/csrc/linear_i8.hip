@@ -95,6 +95,13 @@ __device__ __forceinline__ void li_tile(int block, int tiles_m, int tiles_n, int
     tn = rem / gm;
 }
 
+// Many rows of a product are bound by the clock under load: 32,000 x 25,088 x 1,024 by 256 x 256 tiles takes 684 us,
+// 2.40 POPS, with the matrix pipes busy in 55 % of the cycles at 2.05 GHz (zeros for operands and no traffic: 447 us where
+// this took 712).  At k = 1,024 (to bf16, 45 us) the stores and the 64-bit epilogue, which nothing overlaps with one
+// workgroup a CU, take the larger part; 2,000 x 12,544 x 1,024 by 128 x 128 in two splits takes 38 us and 9 to join.
+// Tried: 32 x 32 x 32 instructions 711 -> 744 us; 128 x 256 tiles in a ring of three stages, two workgroups a CU,
+// 688 -> 874 us (45 -> 50 at k = 1,024); 128 x 128 a wave spills.
+//
 // One tile of BM x BN by waves of WM x WN.  k goes by in stages of 64 bytes: global -> LDS directly, LI_STAGES in the
 // ring; LDS -> registers one stage ahead of the matrix instructions; so that a load has LI_STAGES - 1 stages to arrive.
 template <int BM, int BN, int WM, int WN, int P>
@@ -311,6 +318,9 @@ linear_i8_kernel(const LiArgs A)
     linear_i8_tile<BM, BN, WM, WN, P>(A, blockIdx.x, blockIdx.y);
 }
 
+// Three products of bytes for each of the gradient's: 2,048 x 25,088 x 1,024 (both, 0.63 T operations) 322-351 us,
+// 1.8-2.0 POPS; 8,192 x 1,024 x 1,024 58 us, 1.8 POPS.  64 x 128 tiles, because three sums a result leave registers for no
+// more at two workgroups a CU.
 // Both gradients' products in one launch: the first `blocks` workgroups are A's (tiles of a split next to each other), the
 // rest B's.
 template <int BM, int BN, int WM, int WN, int OCC>
@@ -322,7 +332,9 @@ linear_i8_grad_kernel(const LiArgs A, const LiArgs B, int blocks)
     const int i = second ? blockIdx.x - blocks : blockIdx.x, tiles = R.tiles_m * R.tiles_n;
     linear_i8_tile<BM, BN, WM, WN, 3>(R, i % tiles, i / tiles);
 }
-// Joins the sums of a split k: a lane takes four neighbours.  (Letting the split that arrives last do this, behind a
+
+// Joins the sums of a split k: a lane takes four neighbours.  2,000 x 1,024 of two splits 8.8 us, 2,048 x 1,024 of eight 16 us
+// (4.7 TB/s): bound by the sums' way in.  (Letting the split that arrives last do this, behind a
 // device-scope fence, was tried: the fence writes back the whole L2 and the product of 2,000 x 12,544 x 1,024 went from 44
 // to 165 us.)
 template <int P> __device__ __forceinline__ void linear_i8_join(const LiArgs &A, int64_t i)
@@ -374,7 +386,8 @@ __global__ void __launch_bounds__(64) linear_i8_grad_join_kernel(const LiArgs A,
 // One launch from float rows (or codes) to the result: a workgroup takes LF_N output channels and all of k.  A thread owns
 // the 16-byte chunks t, t + 1024, ... of k, of the weight rows and of x alike, so that it needs nothing of its neighbours but
 // the row's maximum and the final sum; the weights, which are all there is to read, stay in its registers for every row of
-// x.  Each workgroup quantises x for itself, out of the L2.
+// x.  Each workgroup quantises x for itself, out of the L2.  One row of 12,544 by 1,024 channels: 6.4 us for 12.9 MB
+// (2.0 TB/s); a chain of load, maximum over the workgroup, codes and sum over the workgroup bounds it.
 #define LF_THREADS 1024
 #define LF_N 4
 #define LF_CHUNKS 2 // of a thread: k up to 32,768
@@ -481,7 +494,8 @@ linear_i8_few_kernel(const T *__restrict__ x, int64_t x_stride, const float *__r
 // its BM / 8 rows, up to four at a time so that their chains of dependent operations overlap; then it multiplies all BM rows
 // with 16 output channels of its own, whose weights it takes straight from the L2 into registers (no two waves of a workgroup
 // want the same ones), LR_AHEAD steps ahead.  blockIdx.y: a group of output channels; with few rows the groups are what
-// fills the chip, and each quantises for itself.
+// fills the chip, and each quantises for itself.  32,000 rows of 1,024 fp32 by 105 channels: 36.6 us, 145 MB at 4.0 TB/s;
+// a workgroup reads and then multiplies, and two of them a CU overlap only in part.
 #define LR_THREADS 512
 #define LR_K 1024
 #define LR_AHEAD 8
@@ -553,6 +567,7 @@ __device__ __forceinline__ void linear_i8_short(const T *__restrict__ x, int64_t
                 const int k = (kf & ~63) + lane;
                 row[lr_slot(k >> 4, r) * 16 + (k & 15)] = 0;
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // other lanes' codes stay behind these zeros; no instruction
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int k = (i * 64 + lane) * V;

@@ -4,6 +4,8 @@
 
 // One workgroup a row, the row held in registers between the maximum and the codes (V elements of 16 bytes a load,
 // NV loads a thread), so that x is read once.
+// Bound by HBM: 32,000 rows of 25,088 fp32 727 us (4.0 GB, 5.5 TB/s), 2,000 of 12,544 21.6 us (5.8 TB/s), 32,000 of 1,024
+// bf16 18.8 us (5.2 TB/s); a copy of 4 GiB reaches 4.7 TB/s.
 // Two workgroups' rows have to fit a CU, so that one loads while the other computes: registers are bounded to 64.
 template <typename T, int THREADS, int NV>
 __global__ void __launch_bounds__(THREADS, 8)
@@ -175,7 +177,7 @@ template <typename T> __device__ __forceinline__ float gd_grad(const T *grad, co
     return y && (float)y[yi] <= 0.0f ? 0.0f : g;
 }
 
-// Fixed point relative to `top`: T = round(a I8_FIX / top), off by at most top 2^-24; the product and the factor are
+// Fixed point relative to `top`: T = round(a I8_FIX / top), off by at most half a step, 1.008 top 2^-24; the product and the factor are
 // formed in 64 bits.
 __device__ __forceinline__ int gd_fix(float a, double inv) { return (int)__builtin_rint((double)a * inv); }
 
@@ -304,7 +306,7 @@ __device__ __forceinline__ void gd_col_partials(const I8Grad &A, int bx, int by,
 }
 
 // All that depends on nothing but the call's inputs, in one launch: workgroups [0, b0) row digits, [b0, b1) column
-// partials, [b1, b2) b transposed, [b2, b3) a transposed.
+// partials, [b1, b2) b transposed, [b2, b3) a transposed.  2,048 x 25,088 x 1,024 fp32: 40 us, 0.18 GB at 4.5 TB/s.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256)
 grad_prepare_kernel(const I8Grad A, int b0, int b1, int b2)
@@ -332,6 +334,7 @@ grad_prepare_kernel(const I8Grad A, int b0, int b1, int b2)
     }
 }
 
+// 2,048 x 1,024 fp32 12.7 us, 8,192 x 1,024 bf16 21.9 us: the column's partials, one after the other, are waited for first.
 template <typename T>
 __global__ void __launch_bounds__(256)
 grad_col_digits_kernel(const I8Grad A, int n_part)

@@ -540,6 +540,76 @@ def test_other_stream_and_captured_replays(dev):
             same_bits(u, v)
 
 
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1, 300, 2100), (99, 1024, 4100), (700, 400, 2048), (2000, 520, 1030)])
+def test_forms_captured_and_on_two_streams(dev, m, n, k):
+    """One launch, short rows and tiles with a split k: two streams work at once on inputs of their own, and two captured
+    calls are replayed in turn on new inputs, each against the eager result."""
+    from objectdetection_amd import ops
+    wc, ws = ops.quantize_rows_i8(torch.randn((n, k), generator=torch.Generator().manual_seed(9)).to(dev))
+    xs = [features(m, k, 30 + i).to(dev) for i in range(2)]
+    eager = [ops.linear_i8(x, wc, ws, None, True) for x in xs]
+    streams = [torch.cuda.Stream(device=dev) for _ in xs]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.linear_i8(xs[i], wc, ws, None, True))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            same_bits(y, eager[i])
+    graphs, held = [], []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held.append(ops.linear_i8(x, wc, ws, None, True))
+        graphs.append(graph)
+    for r in range(3):
+        for i, x in enumerate(xs):
+            x.copy_(features(m, k, 40 + 2 * r + i).to(dev))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for i, x in enumerate(xs):
+            same_bits(held[i], ops.linear_i8(x, wc, ws, None, True))
+
+
+@gpu
+def test_captured_training_step(dev):
+    """Forward and backward of LinearI8 recorded into one graph and replayed on new inputs and weights."""
+    from objectdetection_amd import ops
+    x = features(130, 300, 3).to(dev).requires_grad_()
+    w = torch.randn((40, 300), generator=torch.Generator().manual_seed(5)).to(dev).requires_grad_()
+    b = torch.randn((40,), generator=torch.Generator().manual_seed(7)).to(dev).requires_grad_()
+    up = torch.randn((130, 40), generator=torch.Generator().manual_seed(6)).to(dev)
+
+    def step():
+        y = ops.LinearI8.apply(x, w, b, True)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), up)
+    side = torch.cuda.Stream(device=dev)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(features(130, 300, 50 + i).to(dev))
+            w.mul_(0.5)
+            up.neg_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        for u, v in zip(got, step()):
+            same_bits(u, v)
+
+
 # ------------------------------------------------------------------------------------------------- the box head
 def _float_head(dev, in_channels=3 * 49, rep=70, classes=5, int8=False):
     from objectdetection_amd.ROIHead import FasterRCNNPredictor, TwoMLPHead
@@ -661,6 +731,23 @@ def test_roi_head_serves_and_trains_through_int8(dev):
         # RoIAlign's backward adds with atomics for maps of this size: the order of its sums is not fixed
         torch.testing.assert_close(a.grad, b.grad, rtol=1e-4, atol=1e-6 * float(b.grad.abs().max()))
     assert head.fc1.weight.grad.abs().sum() > 0 and maps[0].grad.abs().sum() > 0
+
+
+def test_scales_stay_in_32_bits_and_old_modules_load():
+    from objectdetection_amd.ROIHead import FasterRCNNPredictor, Int8Linear, Int8TwoMLPHead, TwoMLPHead
+    scale = torch.full((4,), 1.2345678e-7)
+    for cast in (lambda m: m.half(), lambda m: m.to(BF16), lambda m: m.double(), lambda m: m.float()):
+        layer = Int8Linear(8, 4)
+        layer.scale.copy_(scale)
+        layer = cast(layer)
+        assert layer.scale.dtype == layer.bias.dtype == F32 and layer.codes.dtype == torch.int8
+        assert torch.equal(layer.scale, scale)
+    assert Int8Linear(8, 4, bias=False).half().bias is None
+    head = Int8TwoMLPHead(8, 4).half()
+    assert head.fc1.scale.dtype == F32 and set(dict(head.named_buffers())) == set(head.state_dict())
+    for old in (TwoMLPHead(8, 4), FasterRCNNPredictor(4, 3)):  # as restored from before the choice
+        del old.__dict__["int8"]
+        old(torch.zeros((2, old.fc1.in_features if hasattr(old, "fc1") else 4)))
 
 
 @gpu
