@@ -6,9 +6,10 @@
 // NV loads a thread), so that x is read once.
 // Bound by HBM: 32,000 rows of 25,088 fp32 727 us (4.0 GB, 5.5 TB/s), 2,000 of 12,544 21.6 us (5.8 TB/s), 32,000 of 1,024
 // bf16 18.8 us (5.2 TB/s); a copy of 4 GiB reaches 4.7 TB/s.
-// Two workgroups' rows have to fit a CU, so that one loads while the other computes: registers are bounded to 64.
+// Two workgroups' rows have to fit a CU, so that one loads while the other computes: registers are bounded to 64 (but for
+// the longest rows, 32,000 of 50,176 fp32 1,540 us, 5.2 TB/s).
 template <typename T, int THREADS, int NV>
-__global__ void __launch_bounds__(THREADS, 8)
+__global__ void __launch_bounds__(THREADS, NV > 7 ? 4 : 8)
 quantize_rows_kernel(const I8Rows A, const I8Rows B, int K)
 {
     constexpr int V = 16 / sizeof(T);
@@ -63,23 +64,57 @@ quantize_rows_kernel(const I8Rows A, const I8Rows B, int K)
         cr[kf + t] = (int8_t)(q.none || kf + t >= K ? 0 : qr_code((float)v_tail, q));
 }
 
-// Rows too long for the registers of a workgroup: the same in two passes over the row.
+// Rows too long for the registers of a workgroup: the same in two passes over the row, the second out of the caches.
+// 2,000 rows of 60,000 bf16 102 us (0.36 GB once, 3.5 TB/s), of 131,000 fp32 408 us (3.2 TB/s).
 template <typename T>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(1024, 8)
 quantize_rows_long_kernel(const I8Rows A, int K)
 {
+    constexpr int V = 16 / sizeof(T), AHEAD = 4, STEP = 1024 * V * AHEAD;
     __shared__ uint32_t red[16];
-    const int row = blockIdx.x;
+    const int row = blockIdx.x, t = threadIdx.x;
     if (row >= i8_rows(A.n_rows, A.M)) return;
     const T *xr = (const T *)A.x + (int64_t)row * A.x_stride;
     int8_t *cr = A.codes + (int64_t)row * A.c_stride;
-    uint32_t top_bits = 0;
-    for (int k = threadIdx.x; k < K; k += 1024) top_bits = qr_max(top_bits, qr_bits((float)xr[k]));
+    const int kf = K - K % V; // whole vectors up to here; the last K % V elements one a thread
+    auto load = [&](I8Vec<T, V>(&v)[AHEAD], int k0) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = k0 + (i * 1024 + t) * V;
+            v[i] = I8Vec<T, V>{};
+            if (k < kf) v[i] = i8_load<T, V>(xr + k);
+        }
+    };
+    const T v_tail = kf + t < K && t < V ? xr[kf + t] : (T)0.0f;
+    uint32_t top_bits = qr_bits((float)v_tail);
+    for (int k0 = 0; k0 < kf; k0 += STEP) {
+        I8Vec<T, V> v[AHEAD];
+        load(v, k0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) top_bits = qr_max(top_bits, qr_bits((float)v[i].v[j]));
+    }
     const QrRow q = qr_row(qr_block_max<1024>(top_bits, red));
-    if (threadIdx.x == 0) A.scale[row] = q.scale;
-    const int end = (A.c_stride & 15) == 0 ? (K + 15) & ~15 : K;
-    for (int k = threadIdx.x; k < end; k += 1024)
-        cr[k] = (int8_t)(q.none || k >= K ? 0 : qr_code((float)(q.far ? qr_lift(xr[k], q) : xr[k]), q));
+    if (t == 0) A.scale[row] = q.scale;
+    auto code = [&](T x) { return q.none ? 0 : qr_code((float)(q.far ? qr_lift(x, q) : x), q); };
+    const bool wide = (A.c_stride & 15) == 0;
+    for (int k0 = 0; k0 < kf; k0 += STEP) {
+        I8Vec<T, V> v[AHEAD];
+        load(v, k0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = k0 + (i * 1024 + t) * V;
+            if (k >= kf) break;
+            uint32_t p[V / 4];
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j)
+                p[j] = qr_pack(code(v[i].v[4 * j]), code(v[i].v[4 * j + 1]), code(v[i].v[4 * j + 2]), code(v[i].v[4 * j + 3]));
+            if (wide) __builtin_memcpy(__builtin_assume_aligned(cr + k, V), p, V);
+            else __builtin_memcpy(cr + k, p, V);
+        }
+    }
+    if (t < 16 && kf + t < (wide ? (K + 15) & ~15 : K)) cr[kf + t] = (int8_t)(kf + t >= K ? 0 : code(v_tail));
 }
 
 // B: rows of a second matrix of the same type and length in the same launch (B.M = 0: none)
@@ -105,7 +140,8 @@ template <typename T> static int quantize_rows_t(const I8Rows &A, const I8Rows &
     QR_LAUNCH(1024, 1)
     QR_LAUNCH(1024, 4)
     if constexpr (V == 4) {
-        QR_LAUNCH(1024, 7) // what 64 registers hold
+        QR_LAUNCH(1024, 7)  // what 64 registers hold
+        QR_LAUNCH(1024, 16) // and 128, one workgroup a CU: 2,000 rows of 60,000 145 us, in two passes 176; in 16 bits it spills
     }
 #undef QR_LAUNCH
     for (const I8Rows *r : {&A, &B}) {

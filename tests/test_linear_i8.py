@@ -218,6 +218,34 @@ def test_quantize_ties_and_extremes(dev, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [33001, 65536])
+def test_quantize_long_rows(dev, k, dtype):
+    """Rows that take two passes: extremes, Inf and NaN in the last element, odd offsets, codes on an odd stride."""
+    from objectdetection_amd import _lib, ops
+    fin = torch.finfo(dtype)
+    base = features(8, k + 3, k, torch.float64)
+    base[:, k] = 1.0
+    for i, top in enumerate((fin.max, fin.tiny, fin.tiny * fin.eps * 5, 0.0)):
+        base[i] *= top / base[i].abs().max()
+    base = base.to(dtype)
+    base[4, k], base[5, k] = float("inf"), float("nan")
+    x = base[:, 1:k + 1]
+    ref, ref_scale = plain_codes(x)
+    on = base.to(dev)[:, 1:k + 1]
+    codes, scale = ops.quantize_rows_i8(on)
+    assert torch.equal(codes.cpu().double(), ref)
+    same_bits(scale, ref_scale)
+    odd = torch.full((8, k + 2 - k % 2), 77, dtype=torch.int8, device=dev)
+    P = ctypes.c_void_p
+    n = torch.tensor([7], dtype=torch.int32, device=dev)
+    assert _lib.load().frcnn_quantize_rows_i8(P(on.data_ptr()), ops._I8_TYPES[dtype], on.stride(0), 8, k, P(n.data_ptr()),
+                                              P(odd.data_ptr()), odd.stride(0), P(scale.data_ptr()),
+                                              P(torch.cuda.current_stream().cuda_stream)) == 0
+    assert torch.equal(odd.cpu()[:7, :k].double(), ref[:7]) and (odd[:, k:] == 77).all() and (odd[7] == 77).all()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_quantize_views_and_counts(dev, dtype):
     from objectdetection_amd import ops
