@@ -468,6 +468,14 @@ def test_gradients_against_the_formulas(dev, m, n, k, dtype, wdtype, relu):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(2049, 40, 70), (5003, 33, 130), (70, 2500, 65), (40, 4101, 20), (2300, 2200, 64)])
+def test_gradients_of_long_sums(dev, m, n, k):
+    """Sums over many rows or channels: in one piece, and split over workgroups and joined."""
+    test_gradients_against_the_formulas(dev, m, n, k, F32, F32, True)
+    test_gradients_against_the_formulas(dev, m, n, k, BF16, F32, False)
+
+
+@gpu
 def test_gradients_against_differences(dev):
     """The straight-through gradient is that of f = sum(grad * relu(X W^T + b)) at the dequantised X, W: central
     differences of f in 64 bits, along random directions.  f is piecewise linear in each argument, so away from a kink a
