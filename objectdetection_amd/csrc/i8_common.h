@@ -98,7 +98,7 @@ template <int THREADS> __device__ __forceinline__ uint32_t qr_block_max(uint32_t
 
 // A signed 24-bit fixed-point number T (|T| <= I8_FIX) as three signed 8-bit digits, T = d0 2^16 + d1 2^8 + d2 with
 // d0 in [-127, 127] and d1, d2 in [-128, 127].
-#define I8_FIX 8323072 /* 127 * 2^16 */
+#define I8_FIX (127 << 16)
 __device__ __forceinline__ void i8_digits(int T, int &d0, int &d1, int &d2)
 {
     d0 = (T + 32896) >> 16;
