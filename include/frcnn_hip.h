@@ -369,7 +369,7 @@ int frcnn_resize_pad_batch_f32(const float *const *src_host, const int32_t *shap
 #define FRCNN_BF16 1
 #define FRCNN_F16 2
 
-/* Row quantiser.  x: (M,K), row stride in elements (any, 0 for a broadcast row).  Per row: top = max |x|;
+/* Row quantiser.  x: (M,K), K at most 2^30, row stride in elements (any, 0 for a broadcast row).  Per row: top = max |x|;
  * scale = top / 127 in fp32; code = the whole number nearest to the exact quotient 127 x / top, ties to even (so in
  * [-127, 127]).  A row of zeros has scale 0 and codes 0; a row with an Inf or a NaN has scale NaN and codes 0.
  * n_rows: device int32 count of valid rows (clamped to [0, M]; rows behind it are neither read nor written) or NULL.

@@ -109,6 +109,8 @@ __device__ __forceinline__ void i8_digits(int T, int &d0, int &d1, int &d2)
 
 // Longest contraction: 2^17 - 1 products of at most 2^14 cannot leave 32 bits.
 #define I8_MAX_K 131071
+// Longest row of the quantiser alone: its column indices are 32-bit, and a step of the long-row form past the end stays one
+#define I8_MAX_ROW (1 << 30)
 // Most rows: a launch has fewer than 2^32 threads, up to 1,024 of them a row
 #define I8_MAX_ROWS 4194303
 

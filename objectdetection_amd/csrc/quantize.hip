@@ -167,7 +167,8 @@ extern "C" int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_strid
                                       int8_t *codes, int64_t codes_stride, float *scale, void *stream)
 {
     FRCNN_REQUIRE(i8_type_ok(x_type), "quantize_rows: unknown element type %d", x_type);
-    FRCNN_REQUIRE(M >= 0 && M <= I8_MAX_ROWS && K > 0, "quantize_rows: bad shape (%d, %d); at most %d rows", M, K, I8_MAX_ROWS);
+    FRCNN_REQUIRE(M >= 0 && M <= I8_MAX_ROWS && K > 0 && K <= I8_MAX_ROW,
+                  "quantize_rows: bad shape (%d, %d); at most %d rows of %d", M, K, I8_MAX_ROWS, I8_MAX_ROW);
     FRCNN_REQUIRE(codes_stride >= K && x_stride >= 0, "quantize_rows: bad strides");
     if (M == 0) return FRCNN_OK;
     FRCNN_REQUIRE(x && codes && scale, "quantize_rows: null pointer");

@@ -982,6 +982,8 @@ class MultiScaleRoIAlign(torch.nn.Module):
 # ------------------------------------------------------- 8-bit dense layers of the box head
 _I8_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 I8_MAX_K = 131071  # the 32-bit sums of the product cannot wrap up to here
+I8_MAX_ROW = 1 << 30  # longest row of the quantiser alone
+I8_MAX_ROWS = 4194303  # rows of any matrix
 
 # A layer of a few rows is bound by the host, so these wrappers spend little there: pointers go to ctypes as numbers, the
 # stream comes as a number without a Stream object around it (0.1 us against 1.9), the device is switched only if it is
@@ -1026,13 +1028,21 @@ def _i8_device(what, dev, *tensors):
             raise ValueError("%s: all tensors have to be on %s; got one on %s" % (what, dev, t.device))
 
 
-def _i8_rows(x, what):
+def _i8_sizes(what, M, N, K, longest=I8_MAX_K):
+    """Before a copy, an allocation or a call: ctypes would pass on the low 32 bits of a larger number."""
+    if M > I8_MAX_ROWS or N > I8_MAX_ROWS or K > longest:
+        raise ValueError("%s: %d rows by %d channels, rows of %d; at most %d, %d and %d"
+                         % (what, M, N, K, I8_MAX_ROWS, I8_MAX_ROWS, longest))
+
+
+def _i8_rows(x, what, longest=I8_MAX_K):
     """x (M,K) as a tensor the kernels read in place: one of the three float types, elements of a row next to each
     other, rows any stride apart."""
     if not x.is_cuda:
         _need_gpu(x)
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError("%s expects (M,K) with K > 0; got %s" % (what, tuple(x.shape)))
+    _i8_sizes(what, x.shape[0], 1, x.shape[1], longest)
     if x.dtype not in _I8_TYPES:
         x = x.detach().to(torch.float32)
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.detach().contiguous()
@@ -1066,20 +1076,20 @@ def _i8_weights(codes, scale, bias, K, dev, what):
     if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[0] == 0 or codes.shape[1] != K:
         raise ValueError("%s expects weight codes (N,%d) int8; got %s %s" % (what, K, tuple(codes.shape), codes.dtype))
     N = codes.shape[0]
+    _i8_sizes(what, 0, N, K)
     if scale.dim() != 1 or scale.shape[0] != N or (bias is not None and (bias.dim() != 1 or bias.shape[0] != N)):
         raise ValueError("%s expects a scale and a bias for each of the %d outputs" % (what, N))
-    if K > I8_MAX_K:
-        raise ValueError("%s: rows of %d; at most %d" % (what, K, I8_MAX_K))
     return N, _i8_codes(codes), _f32v(scale), _f32v(bias)
 
 
 def quantize_rows_i8(x, n_rows=None):
     """Rows of x (M,K; fp32, bf16 or fp16) as 8-bit integers: scale (M) = max |x| / 127 in fp32, codes (M,K) int8 = the
     whole numbers nearest to 127 x / max |x| (of the exact quotient, ties to even), so that x ~ codes * scale[:, None].
+    At most 4,194,303 rows of up to 2^30 elements.
     A row of zeros: scale 0, codes 0; a row with an Inf or a NaN: scale NaN, codes 0.  n_rows (1) int32 on the device:
     rows behind it are left out (their outputs are unspecified), as in the padded RoI path.  Rows of the codes lie a
     multiple of 16 bytes apart, the form matmul_i8 reads in place."""
-    x = _i8_rows(x, "quantize_rows_i8")
+    x = _i8_rows(x, "quantize_rows_i8", I8_MAX_ROW)
     M, K = x.shape
     dev = x.device
     n_rows = _i8_count(n_rows, "quantize_rows_i8", dev)
@@ -1101,6 +1111,7 @@ def matmul_i8(codes, scale, weight_codes, weight_scale, bias=None, relu=False, o
     if out_dtype not in _I8_TYPES:
         raise ValueError("matmul_i8: out_dtype is float32, bfloat16 or float16; got %s" % out_dtype)
     M, K = codes.shape
+    _i8_sizes("matmul_i8", M, 1, K)
     dev = codes.device
     _i8_device("matmul_i8", dev, scale)
     N, weight_codes, weight_scale, bias = _i8_weights(weight_codes, weight_scale, bias, K, dev, "matmul_i8")
