@@ -415,9 +415,9 @@ int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride, const voi
  * a ReLU, NULL otherwise):
  *   grad_x[m,k] = sum_n g[m,n] b_scale[n] b[n,k]     grad_w[n,k] = sum_m g[m,n] a_scale[m] a[m,k]
  *   grad_bias[n] = sum_m g[m,n]  (fp32, summed in a fixed order)
- * The factors g b_scale and g a_scale are taken as 24-bit fixed-point numbers relative to the largest of their row m
- * (grad_x) or column n (grad_w), and the sums over them are exact: a factor is rounded to fp32 and then to fixed point, so
- * an output is off by at most 2.01 * 2^-24 max|factor| sum|code| before its rounding.  An Inf or a NaN among a row's (column's) factors makes that whole
+ * Each factor g b_scale and g a_scale is held to 2^-23 of itself, or to 2^-50 of the largest of its row m (grad_x) or
+ * column n (grad_w), whichever is more; its product with a code is exact and the sums are fp32, so an output is off by what
+ * an fp32 product of the same factors is.  An Inf or a NaN among a row's (column's) factors makes that whole
  * row of grad_x (grad_w) NaN.  grad_x / grad_w: contiguous; grad_x, grad_w, grad_bias: NULL where not wanted.
  * M, N, K <= 131071.  The results have the same bits every run. */
 size_t frcnn_linear_i8_backward_workspace_bytes(int M, int N, int K);

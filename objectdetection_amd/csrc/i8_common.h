@@ -96,15 +96,23 @@ template <int THREADS> __device__ __forceinline__ uint32_t qr_block_max(uint32_t
     return v;
 }
 
-// A signed 24-bit fixed-point number T (|T| <= I8_FIX) as three signed 8-bit digits, T = d0 2^16 + d1 2^8 + d2 with
-// d0 in [-127, 127] and d1, d2 in [-128, 127].
-#define I8_FIX (127 << 16)
-__device__ __forceinline__ void i8_digits(int T, int &d0, int &d1, int &d2)
+// A gradient's factor f of a row whose largest magnitude is `top`, as two fp16 numbers: v = f 2^i8_shift(top), |v| < 2^15;
+// hi = v in fp16, lo = (v - hi) 2^12 in fp16, so that v ~ hi + lo 2^-12.  hi is off by at most 2^-11 of v's power of two and
+// lo by 2^-12 of what is left, so f is off by at most 2^-23 of ITSELF down to 2^-27 of top (from there hi is a subnormal
+// number), and by 2^-50 of top below.  A product with an 8-bit code (also fp16) is exact in fp32.
+// Rounding to 23 bits is a choice: all 24 take a third piece, half as much again of the matrix instructions, for an error
+// that the sums' own roundings in fp32 hide; fixed point relative to top, in three signed 8-bit digits on the integer
+// instructions, takes three quarters of the time and loses the factors far below top: against a confident classifier's
+// cross-entropy gradients one entry of dL/dw in a hundred was off by a fifth of itself.
+// (top comes to [2^13, 2^14): the exact product may lie half above a top that is a subnormal fp32 number, and lo must not
+// overflow.)
+#define I8_LO 4096.0
+__device__ __forceinline__ int i8_shift(float top) { return 14 - __builtin_amdgcn_frexp_expf(top); }
+__device__ __forceinline__ double i8_pow2(int e) { return __builtin_amdgcn_ldexp(1.0, e); }
+__device__ __forceinline__ void i8_pieces(double v, _Float16 &hi, _Float16 &lo)
 {
-    d0 = (T + 32896) >> 16;
-    const int r = T - (d0 << 16); // in [-32896, 32639]
-    d1 = (r + 128) >> 8;
-    d2 = r - (d1 << 8);
+    hi = (_Float16)(float)v;
+    lo = (_Float16)(float)((v - (double)(float)hi) * I8_LO);
 }
 
 // Longest contraction: 2^17 - 1 products of at most 2^14 cannot leave 32 bits.
@@ -138,13 +146,13 @@ struct I8Grad { // a training step's backward inputs, and what its products read
     int64_t a_stride, b_stride;
     const float *a_scale, *b_scale;
     int M, N, K;
-    // dL/dx: digits (3, M, row_stride) of g b_scale, their magnitudes (M), b transposed (K, row_stride); NULL: not wanted
-    int8_t *row_digits, *b_t;
+    // dL/dx: pieces (2, M, row_stride) of g b_scale, their magnitudes (M), b transposed (K, row_stride); NULL: not wanted
+    _Float16 *row_pieces, *b_t;
     float *row_top;
     int64_t row_stride;
-    // dL/dw: digits (3, N, col_stride) of g a_scale, their magnitudes (N), a transposed (K, col_stride; NULL: only
+    // dL/dw: pieces (2, N, col_stride) of g a_scale, their magnitudes (N), a transposed (K, col_stride; NULL: only
     // dL/dbias wanted), partial magnitudes and sums of the columns (frcnn_i8_grad_parts(M), N)
-    int8_t *col_digits, *a_t;
+    _Float16 *col_pieces, *a_t;
     float *col_top;
     int64_t col_stride;
     uint32_t *part_top;

@@ -1,14 +1,16 @@
 // linear_i8.hip -- dense layers on 8-bit integers: out_mn = (sum_k a_mk b_nk) a_scale_m b_scale_n + bias_n, rows of a
-// (RoIs) and rows of b (output channels) both contiguous in k, and the two gradient products, which are the same
-// product on 24-bit fixed-point gradients (three 8-bit digits, three sums).
+// (RoIs) and rows of b (output channels) both contiguous in k, and the two gradient products, which go through the same
+// tiles in fp16: a gradient's factor in two pieces (i8_pieces), a code as it is, sums in fp32 that are joined in 64 bits.
 //
-// The sums are exact: 32-bit integers cannot wrap below 2^17 products of two bytes.  Their order therefore does not
-// matter, and splitting k over workgroups changes no bit.  The scales and the bias are applied in 64 bits and the
+// The layer's sums are exact: 32-bit integers cannot wrap below 2^17 products of two bytes.  Their order therefore does
+// not matter, and splitting k over workgroups changes no bit.  The gradients' sums have one fixed order for a size.  The scales and the bias are applied in 64 bits and the
 // result is rounded to fp32 (and from there to 16 bits): the sign a ReLU looks at is the sign of the exact expression.
 #include "i8_common.h"
 #include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 #define LI_BK 64           // bytes of k per LDS stage: one matrix instruction deep
@@ -20,14 +22,14 @@ struct LiArgs {
     const int8_t *a, *b;
     int64_t a_stride, b_stride, a_plane; // bytes
     const int32_t *n_rows;               // device count of valid rows of a, or NULL
-    int M, N, K;
+    int M, N, K;                         // K: bytes of a row's k (two pieces: two a number, zeros up to a multiple of 32)
     int tiles_m, tiles_n, k_split;       // k_split: bytes of k per split, a multiple of LI_BK
     const float *a_scale, *b_scale, *bias;
     int relu, out_type;
     bool stream;                         // results stored past the caches
     void *out;
     int64_t out_stride;                  // elements
-    void *partial;                       // sums of a split k, (splits, M, li_ld4(N)) int32 (P = 3: int64), or NULL
+    void *partial;                       // sums of a split k, (splits, M, li_ld4(N)) int32 (P = 2: double), or NULL
     int splits;
     int n_group;                         // short rows: output channels of a workgroup
 };
@@ -42,11 +44,23 @@ __device__ __forceinline__ float li_finish(double sum, double a_scale, double b_
     return relu && z < 0.0f ? 0.0f : z; // keeps NaN
 }
 
-// sum_p digit_p 2^(8 (2 - p)) of a fixed-point row, or the plain sum
-template <int P> __device__ __forceinline__ double li_sum(int d0, int d1, int d2)
+// P: planes of a.  1: bytes, whole-number sums.  2: the pieces of a gradient's factor, fp32 sums.
+template <int P> struct LiAcc { typedef i32x4 type; };
+template <> struct LiAcc<2> { typedef f32x4 type; };
+__device__ __forceinline__ double li_sum(int s) { return (double)s; }
+__device__ __forceinline__ double li_sum(float hi, float lo) { return __builtin_fma((double)lo, 1.0 / I8_LO, (double)hi); }
+
+// One step of a tile, 64 bytes of k
+__device__ __forceinline__ i32x4 li_mfma(i32x4 b, i32x4 a, i32x4 acc) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, acc, 0, 0, 0); }
+__device__ __forceinline__ f32x4 li_mfma(i32x4 b, i32x4 a, f32x4 acc)
 {
-    const double t = (double)d0;
-    return P == 1 ? t : __builtin_fma(t, 65536.0, __builtin_fma((double)d1, 256.0, (double)d2));
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), acc, 0, 0, 0);
+}
+
+// What a row's sum is multiplied by: its scale, or the way back from i8_shift (NaN for a row that is not finite)
+template <int P> __device__ __forceinline__ double li_row_scale(float s)
+{
+    return P == 1 || s != s ? (double)s : i8_pow2(-i8_shift(s));
 }
 
 // V neighbours (the first `count` of them) in out's type; the address is aligned to one element.  STREAM: past the caches;
@@ -186,13 +200,14 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
     };
     const int wm0 = (wave % (BM / WM)) * WM, wn0 = (wave / (BM / WM)) * WN;
     const int i16 = lane & 15, q4 = lane >> 4;
-    i32x4 acc[P][TM][TN];
+    typedef typename LiAcc<P>::type Acc;
+    Acc acc[P][TM][TN];
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm)
 #pragma unroll
-            for (int tn = 0; tn < TN; ++tn) acc[p][tm][tn] = (i32x4){0, 0, 0, 0};
+            for (int tn = 0; tn < TN; ++tn) acc[p][tm][tn] = (Acc){0, 0, 0, 0};
     // b is the instruction's row operand: a lane's four results are neighbours in n
     const int frag = i16 * BK + ((q4 ^ li_swz(i16)) << 4);
     struct Frags {
@@ -215,7 +230,7 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
         for (int t = 0; t < G; ++t) {
 #pragma unroll
             for (int tn = 0; tn < TN; ++tn)
-                acc[t / TM][t % TM][tn] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.b[tn], f.a[t], acc[t / TM][t % TM][tn], 0, 0, 0);
+                acc[t / TM][t % TM][tn] = li_mfma(f.b[tn], f.a[t], acc[t / TM][t % TM][tn]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = t * R; i < (t + 1) * R && i < P * TM + TN; ++i) read1(g, next, i);
@@ -244,6 +259,10 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the fills past the end, before the LDS is given back
 
+    auto sum = [&](int tm, int tn, int r) {
+        if constexpr (P == 1) return li_sum(acc[0][tm][tn][r]);
+        else return li_sum(acc[0][tm][tn][r], acc[1][tm][tn][r]);
+    };
     const int mw = m0 + wm0 + i16, nw = n0 + wn0 + q4 * 4;
     if (A.splits > 1) {
 #pragma unroll
@@ -255,15 +274,13 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
                 const int n = nw + tn * 16;
                 if (n >= A.N) continue;
                 const int64_t at = ((int64_t)split * A.M + m) * li_ld4(A.N) + n;
-                if (P == 1) {
+                if constexpr (P == 1) {
                     *(i32x4 *)((int32_t *)A.partial + at) = acc[0][tm][tn];
                 } else {
-                    int64_t v[4];
+                    double v[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        v[r] = ((int64_t)acc[0][tm][tn][r] << 16) + ((int64_t)acc[P > 1 ? 1 : 0][tm][tn][r] << 8) +
-                               acc[P > 2 ? 2 : 0][tm][tn][r];
-                    __builtin_memcpy(__builtin_assume_aligned((int64_t *)A.partial + at, 16), v, 32);
+                    for (int r = 0; r < 4; ++r) v[r] = sum(tm, tn, r);
+                    __builtin_memcpy(__builtin_assume_aligned((double *)A.partial + at, 16), v, 32);
                 }
             }
         }
@@ -271,10 +288,7 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
     }
     double sa[TM];
 #pragma unroll
-    for (int tm = 0; tm < TM; ++tm) {
-        sa[tm] = mw + tm * 16 < M ? (double)A.a_scale[mw + tm * 16] : 0.0;
-        if (P == 3) sa[tm] *= 1.0 / (double)I8_FIX;
-    }
+    for (int tm = 0; tm < TM; ++tm) sa[tm] = mw + tm * 16 < M ? li_row_scale<P>(A.a_scale[mw + tm * 16]) : 0.0;
     auto write = [&](auto *out, auto stream) {
         constexpr int PT = sizeof(*out) == 2 && TN % 2 == 0 ? 2 : 1, V = 4 * PT; // tiles a store takes
 #pragma unroll
@@ -292,11 +306,7 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
                 const int m = mw + tm * 16;
                 float z[V];
 #pragma unroll
-                for (int r = 0; r < V; ++r) {
-                    const int t = tn + r / 4, e = r % 4;
-                    z[r] = li_finish(li_sum<P>(acc[0][tm][t][e], acc[P > 1 ? 1 : 0][tm][t][e], acc[P > 2 ? 2 : 0][tm][t][e]),
-                                     sa[tm], sb[r], bias[r], A.relu);
-                }
+                for (int r = 0; r < V; ++r) z[r] = li_finish(sum(tm, tn + r / 4, r % 4), sa[tm], sb[r], bias[r], A.relu);
                 if (m < M) li_store<decltype(stream)::value>(out + (int64_t)m * A.out_stride + n, z, A.N - n);
             }
         }
@@ -318,9 +328,9 @@ linear_i8_kernel(const LiArgs A)
     linear_i8_tile<BM, BN, WM, WN, P>(A, blockIdx.x, blockIdx.y);
 }
 
-// Three products of bytes for each of the gradient's: 2,048 x 25,088 x 1,024 (both, 0.63 T operations) 322-351 us,
-// 1.8-2.0 POPS; 8,192 x 1,024 x 1,024 58 us, 1.8 POPS.  64 x 128 tiles, because three sums a result leave registers for no
-// more at two workgroups a CU.
+// Two fp16 products for each of the gradient's: 2,048 x 25,088 x 1,024 (both, 0.42 TFLOP) 390-440 us, 0.95-1.08 PFLOP/s, by
+// 128 x 256 (the registers and the LDS of the layer's 256 x 256, whose matrix instructions take as long); 8,192 x 1,024 x
+// 1,024 82 us, 0.84 PFLOP/s, by 64 x 128.  A large library product in fp16 reaches 1.15 PFLOP/s.
 // Both gradients' products in one launch: the first `blocks` workgroups are A's (tiles of a split next to each other), the
 // rest B's.
 template <int BM, int BN, int WM, int WN, int OCC>
@@ -330,7 +340,7 @@ linear_i8_grad_kernel(const LiArgs A, const LiArgs B, int blocks)
     const bool second = (int)blockIdx.x >= blocks;
     const LiArgs &R = second ? B : A;
     const int i = second ? blockIdx.x - blocks : blockIdx.x, tiles = R.tiles_m * R.tiles_n;
-    linear_i8_tile<BM, BN, WM, WN, 3>(R, i % tiles, i / tiles);
+    linear_i8_tile<BM, BN, WM, WN, 2>(R, i % tiles, i / tiles);
 }
 
 // Joins the sums of a split k: a lane takes four neighbours.  2,000 x 1,024 of two splits 8.8 us, 2,048 x 1,024 of eight 16 us
@@ -343,21 +353,22 @@ template <int P> __device__ __forceinline__ void linear_i8_join(const LiArgs &A,
     const int m = (int)(i / quads), n = (int)(i % quads) * 4;
     if (m >= i8_rows(A.n_rows, A.M)) return;
     const int64_t step = (int64_t)A.M * quads;
-    int64_t t[4] = {0, 0, 0, 0};
+    typedef typename std::conditional<P == 1, int64_t, double>::type Sum;
+    Sum t[4] = {0, 0, 0, 0};
 #pragma unroll 8
     for (int k = 0; k < A.splits; ++k) {
-        if (P == 1) {
+        if constexpr (P == 1) {
             const i32x4 v = ((const i32x4 *)A.partial)[k * step + i];
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[r] += v[r];
         } else {
-            int64_t v[4];
-            __builtin_memcpy(v, __builtin_assume_aligned((const int64_t *)A.partial + (k * step + i) * 4, 16), 32);
+            double v[4];
+            __builtin_memcpy(v, __builtin_assume_aligned((const double *)A.partial + (k * step + i) * 4, 16), 32);
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[r] += v[r];
         }
     }
-    const double a_scale = (double)A.a_scale[m] * (P == 3 ? 1.0 / (double)I8_FIX : 1.0);
+    const double a_scale = li_row_scale<P>(A.a_scale[m]);
     float z[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -379,7 +390,7 @@ __global__ void __launch_bounds__(64) linear_i8_join_kernel(const LiArgs A)
 __global__ void __launch_bounds__(64) linear_i8_grad_join_kernel(const LiArgs A, const LiArgs B, int blocks)
 {
     const bool second = (int)blockIdx.x >= blocks;
-    linear_i8_join<3>(second ? B : A, (int64_t)(second ? blockIdx.x - blocks : blockIdx.x) * 64 + threadIdx.x);
+    linear_i8_join<2>(second ? B : A, (int64_t)(second ? blockIdx.x - blocks : blockIdx.x) * 64 + threadIdx.x);
 }
 
 // ---- a few rows -----------------------------------------------------------------------------------------------------
@@ -725,9 +736,19 @@ static LiPlan li_plan(int M, int N, int K)
     return best;
 }
 
-// The gradients' tiles: of the same size for both products, so that one launch takes them.
-static LiPlan li_grad_plan(int rows, int cols, int inner)
+// The gradients' tiles: of the same size for both products, so that one launch takes them.  128 x 256 where the two of them
+// have 512 such tiles, else 64 x 128.  A whole backward call, us, large : small tiles, M x N x K: 2,048 x 1,024 x 25,088
+// 464 : 536, 256 x 1,024 x 25,088 114 : 124, 512 x 1,024 x 12,544 99 : 107, 8,192 x 256 x 4,096 159 : 169; with fewer tiles
+// 8,192 x 1,024 x 1,024 144 : 143, 2,048 x 1,024 x 1,024 92 : 58; and with one row of tiles only, 128 x 1,024 x 25,088,
+// 110 : 96.
+static bool li_grad_large(int M, int N, int K)
 {
+    return M >= 256 && ((int64_t)((M + 127) / 128) + (N + 127) / 128) * ((K + 255) / 256) >= 512;
+}
+
+static LiPlan li_grad_plan(int rows, int cols, int inner, bool large)
+{
+    if (large) return li_split(128, 256, rows, cols, inner, 256 / ((int64_t)((rows + 127) / 128) * ((cols + 255) / 256)));
     const int bn = cols > 64 ? 128 : 64;
     const int64_t tiles = (int64_t)((rows + 63) / 64) * ((cols + bn - 1) / bn);
     return li_split(64, bn, rows, cols, inner, 256 / tiles, LI_SMALL);
@@ -770,7 +791,9 @@ static int li_launch(LiArgs &A, const LiPlan &p, void *split, hipStream_t st)
 static int li_grad_launch(const LiArgs &A, const LiArgs &B, int bn, hipStream_t st)
 {
     const int64_t a = A.out ? (int64_t)A.tiles_m * A.tiles_n * A.splits : 0, b = B.out ? (int64_t)B.tiles_m * B.tiles_n * B.splits : 0;
-    if (bn == 128)
+    if (bn == 256)
+        hipLaunchKernelGGL((linear_i8_grad_kernel<128, 256, 64, 64, 2>), dim3((unsigned)(a + b)), dim3(512), 0, st, A, B, (int)a);
+    else if (bn == 128)
         hipLaunchKernelGGL((linear_i8_grad_kernel<64, 128, 32, 64, 2>), dim3((unsigned)(a + b)), dim3(256), 0, st, A, B, (int)a);
     else
         hipLaunchKernelGGL((linear_i8_grad_kernel<64, 64, 32, 32, 1>), dim3((unsigned)(a + b)), dim3(256), 0, st, A, B, (int)a);
@@ -1015,7 +1038,7 @@ extern "C" int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride
 
 // Workspace of the gradients, part by part
 struct LiGrad {
-    size_t x_split, x_digits, x_top, b_t, w_split, w_digits, w_top, a_t, part_top, part_sum, total;
+    size_t x_split, x_pieces, x_top, b_t, w_split, w_pieces, w_top, a_t, part_top, part_sum, total;
     LiPlan x, w;
 };
 
@@ -1024,20 +1047,31 @@ static LiGrad li_grad(int M, int N, int K)
     LiGrad g;
     const size_t ldn = (size_t)li_stride(N), ldm = (size_t)li_stride(M), parts = (size_t)frcnn_i8_grad_parts(M) * N * 4;
     size_t off = 0;
-    g.x = li_grad_plan(M, K, N);
-    g.w = li_grad_plan(N, K, M);
+    const bool large = li_grad_large(M, N, K);
+    g.x = li_grad_plan(M, K, 2 * (int)ldn, large);
+    g.w = li_grad_plan(N, K, 2 * (int)ldm, large);
     g.x_split = off; off += li_split_bytes(g.x, M, K, 8);
-    g.x_digits = off; off += up256(3 * (size_t)M * ldn);
+    g.x_pieces = off; off += up256(2 * 2 * (size_t)M * ldn);
     g.x_top = off; off += up256((size_t)M * 4);
-    g.b_t = off; off += up256((size_t)K * ldn);
+    g.b_t = off; off += up256(2 * (size_t)K * ldn);
     g.w_split = off; off += li_split_bytes(g.w, N, K, 8);
-    g.w_digits = off; off += up256(3 * (size_t)N * ldm);
+    g.w_pieces = off; off += up256(2 * 2 * (size_t)N * ldm);
     g.w_top = off; off += up256((size_t)N * 4);
-    g.a_t = off; off += up256((size_t)K * ldm);
+    g.a_t = off; off += up256(2 * (size_t)K * ldm);
     g.part_top = off; off += up256(parts);
     g.part_sum = off; off += up256(parts);
     g.total = off;
     return g;
+}
+
+// out (rows, cols) from pieces (2, rows, ld) and codes (cols, ld), both fp16
+static LiArgs li_grad_args(const _Float16 *pieces, const float *top, const _Float16 *codes, int rows, int cols, int64_t ld,
+                           void *out, int out_type)
+{
+    LiArgs A = li_args((const int8_t *)pieces, 2 * ld, top, (const int8_t *)codes, 2 * ld, nullptr, nullptr, 0, rows, cols,
+                       2 * (int)ld, nullptr, out, out_type, cols);
+    A.a_plane = 2 * ld * rows;
+    return A;
 }
 
 extern "C" size_t frcnn_linear_i8_backward_workspace_bytes(int M, int N, int K)
@@ -1077,24 +1111,22 @@ extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t
     g.row_stride = ldn; g.col_stride = ldm;
     LiArgs X = {}, W = {};
     if (grad_x) {
-        g.row_digits = (int8_t *)(ws + l.x_digits);
+        g.row_pieces = (_Float16 *)(ws + l.x_pieces);
         g.row_top = (float *)(ws + l.x_top);
-        g.b_t = (int8_t *)(ws + l.b_t);
-        X = li_args(g.row_digits, ldn, g.row_top, g.b_t, ldn, nullptr, nullptr, 0, M, K, N, nullptr, grad_x, grad_x_type, K);
-        X.a_plane = M * ldn;
+        g.b_t = (_Float16 *)(ws + l.b_t);
+        X = li_grad_args(g.row_pieces, g.row_top, g.b_t, M, K, ldn, grad_x, grad_x_type);
         li_apply(X, l.x, ws + l.x_split);
     }
     if (grad_w || grad_bias) { // the bias gradient is a by-product of the columns' magnitudes
-        g.col_digits = (int8_t *)(ws + l.w_digits);
+        g.col_pieces = (_Float16 *)(ws + l.w_pieces);
         g.col_top = (float *)(ws + l.w_top);
         g.part_top = (uint32_t *)(ws + l.part_top);
         g.part_sum = (float *)(ws + l.part_sum);
         g.grad_bias = grad_bias;
     }
     if (grad_w) {
-        g.a_t = (int8_t *)(ws + l.a_t);
-        W = li_args(g.col_digits, ldm, g.col_top, g.a_t, ldm, nullptr, nullptr, 0, N, K, M, nullptr, grad_w, grad_w_type, K);
-        W.a_plane = N * ldm;
+        g.a_t = (_Float16 *)(ws + l.a_t);
+        W = li_grad_args(g.col_pieces, g.col_top, g.a_t, N, K, ldm, grad_w, grad_w_type);
         li_apply(W, l.w, ws + l.w_split);
     }
     const int rc = frcnn_i8_grad_prepare(g, st);

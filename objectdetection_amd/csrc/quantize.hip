@@ -1,5 +1,5 @@
 // quantize.hip -- what turns rows of numbers into 8-bit integers for linear_i8.hip: the row quantiser, and for the
-// training step the byte transpose and the digits of the gradients.
+// training step the transposed codes and the pieces of the gradients.
 #include "i8_common.h"
 
 // One workgroup a row, the row held in registers between the maximum and the codes (V elements of 16 bytes a load,
@@ -214,12 +214,8 @@ template <typename T> __device__ __forceinline__ float gd_grad(const T *grad, co
     return y && (float)y[yi] <= 0.0f ? 0.0f : g;
 }
 
-// Fixed point relative to `top`: T = round(a I8_FIX / top), off by at most half a step, 1.008 top 2^-24; the product and the factor are
-// formed in 64 bits.
-__device__ __forceinline__ int gd_fix(float a, double inv) { return (int)__builtin_rint((double)a * inv); }
-
-// Byte transpose (rows, cols) -> (cols, rows), one 64 x 64 tile; a thread reads 16 bytes of a row and writes 16 of a column.
-__device__ __forceinline__ void gd_transpose(const int8_t *src, int64_t s_stride, int rows, int cols, int8_t *dst,
+// Codes (rows, cols) -> fp16 (cols, rows), one 64 x 64 tile; a thread reads 16 codes of a row and writes 16 of a column.
+__device__ __forceinline__ void gd_transpose(const int8_t *src, int64_t s_stride, int rows, int cols, _Float16 *dst,
                                              int64_t d_stride, int64_t r0, int64_t c0, int8_t (&tile)[64][68])
 {
     const int tr = threadIdx.x >> 2, tc = (threadIdx.x & 3) * 16;
@@ -237,73 +233,84 @@ __device__ __forceinline__ void gd_transpose(const int8_t *src, int64_t s_stride
     __syncthreads();
     // thread: column tr of the tile, rows tc .. tc + 15
     if (c0 + tr >= cols || r0 + tc >= d_stride) return;
-    for (int j = 0; j < 4; ++j)
-        w[j] = qr_pack(tile[tc + 4 * j][tr], tile[tc + 4 * j + 1][tr], tile[tc + 4 * j + 2][tr], tile[tc + 4 * j + 3][tr]);
-    *(uint4 *)(dst + (c0 + tr) * d_stride + r0 + tc) = make_uint4(w[0], w[1], w[2], w[3]);
+    I8Vec<_Float16, 16> h;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) h.v[j] = (_Float16)(int16_t)tile[tc + j][tr];
+    __builtin_memcpy(__builtin_assume_aligned(dst + (c0 + tr) * d_stride + r0 + tc, 32), &h, 32);
 }
 
-// For dL/dx: a_mn = g_mn * b_scale_n, fixed point relative to the row's largest magnitude.  One wave a row, four
-// neighbours a lane, up to NV of those held in registers; a longer row is read again (from the caches) for its digits.
+// For dL/dx: a_mn = g_mn * b_scale_n in pieces, scaled by the row's largest magnitude.  One wave a row, four neighbours a
+// lane, up to NV of those held in registers; a longer row is read again (from the caches) for its pieces.  The largest is that
+// of the products in fp32, the pieces are taken from the exact products.
 template <typename T, int NV>
-__device__ __forceinline__ void gd_row_digits(const I8Grad &A, int64_t row)
+__device__ __forceinline__ void gd_row_pieces(const I8Grad &A, int64_t row)
 {
     const int lane = threadIdx.x & 63, N = A.N;
     if (row >= A.M) return;
     const T *g = (const T *)A.grad + row * A.grad_stride, *z = A.y ? (const T *)A.y + row * A.y_stride : nullptr;
-    auto load = [&](float(&a)[4], int n) {
+    struct Quad {
+        float g[4], s[4];
+    };
+    auto load = [&](Quad &a, int n) {
         if (n + 4 <= N) {
             const I8Vec<T, 4> v = i8_load<T, 4>(g + n);
             const I8Vec<float, 4> c = i8_load<float, 4>(A.b_scale + n);
             I8Vec<T, 4> u = v;
             if (z) u = i8_load<T, 4>(z + n);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] = (z && (float)u.v[j] <= 0.0f ? 0.0f : (float)v.v[j]) * c.v[j];
+            for (int j = 0; j < 4; ++j) {
+                a.g[j] = z && (float)u.v[j] <= 0.0f ? 0.0f : (float)v.v[j];
+                a.s[j] = c.v[j];
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] = n + j < N ? gd_grad(g, z, n + j, n + j) * A.b_scale[n + j] : 0.0f;
+            for (int j = 0; j < 4; ++j) {
+                a.g[j] = n + j < N ? gd_grad(g, z, n + j, n + j) : 0.0f;
+                a.s[j] = n + j < N ? A.b_scale[n + j] : 0.0f;
+            }
         }
     };
-    float a[NV][4];
+    Quad a[NV];
     uint32_t top_bits = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) load(a[i], (i * 64 + lane) * 4);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top_bits = qr_max(top_bits, qr_bits(a[i][j]));
+        for (int j = 0; j < 4; ++j) top_bits = qr_max(top_bits, qr_bits(a[i].g[j] * a[i].s[j]));
     for (int n = (NV * 64 + lane) * 4; n < N; n += 256) {
-        float t[4];
+        Quad t;
         load(t, n);
-        for (int j = 0; j < 4; ++j) top_bits = qr_max(top_bits, qr_bits(t[j]));
+        for (int j = 0; j < 4; ++j) top_bits = qr_max(top_bits, qr_bits(t.g[j] * t.s[j]));
     }
     for (int o = 32; o > 0; o >>= 1) top_bits = qr_max(top_bits, __shfl_xor(top_bits, o));
     const bool finite = top_bits < 0x7f800000u;
     const float top = __uint_as_float(top_bits);
     const bool none = !finite || top_bits == 0;
-    const double inv = none ? 0.0 : (double)I8_FIX / (double)top;
+    const double up = i8_pow2(i8_shift(top));
     if (lane == 0) A.row_top[row] = finite ? top : __builtin_nanf("");
-    int8_t *d = A.row_digits + row * A.row_stride;
+    _Float16 *d = A.row_pieces + row * A.row_stride;
     const int64_t plane = A.M * A.row_stride;
-    auto store = [&](const float(&t)[4], int n) {
-        int q[3][4];
+    auto store = [&](const Quad &t, int n) {
+        I8Vec<_Float16, 4> h[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) i8_digits(none ? 0 : gd_fix(t[j], inv), q[0][j], q[1][j], q[2][j]);
+        for (int j = 0; j < 4; ++j) i8_pieces(none ? 0.0 : (double)t.g[j] * (double)t.s[j] * up, h[0].v[j], h[1].v[j]);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) *(uint32_t *)(d + p * plane + n) = qr_pack(q[p][0], q[p][1], q[p][2], q[p][3]);
+        for (int p = 0; p < 2; ++p) __builtin_memcpy(__builtin_assume_aligned(d + p * plane + n, 8), &h[p], 8);
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i)
         if ((i * 64 + lane) * 4 < (int)A.row_stride) store(a[i], (i * 64 + lane) * 4);
     for (int n = (NV * 64 + lane) * 4; n < (int)A.row_stride; n += 256) {
-        float t[4];
+        Quad t;
         load(t, n);
         store(t, n);
     }
 }
 
-// For dL/dw: a_mn = g_mn * a_scale_m, fixed point relative to the COLUMN's largest magnitude, written transposed (n, m).
-// First the largest magnitude and the plain sum (dL/dbias) of every column over GC_ROWS rows; then (grad_col_digits_kernel)
-// the column's magnitude from those partials, the digits, and the sum of the partials in row order (the same bits every
+// For dL/dw: a_mn = g_mn * a_scale_m in pieces, scaled by the COLUMN's largest magnitude, written transposed (n, m).
+// First the largest magnitude and the plain sum (dL/dbias) of every column over GC_ROWS rows; then (grad_col_pieces_kernel)
+// the column's magnitude from those partials, the pieces, and the sum of the partials in row order (the same bits every
 // run).
 #define GC_ROWS 64
 template <typename T>
@@ -342,8 +349,8 @@ __device__ __forceinline__ void gd_col_partials(const I8Grad &A, int bx, int by,
     }
 }
 
-// All that depends on nothing but the call's inputs, in one launch: workgroups [0, b0) row digits, [b0, b1) column
-// partials, [b1, b2) b transposed, [b2, b3) a transposed.  2,048 x 25,088 x 1,024 fp32: 40 us, 0.18 GB at 4.5 TB/s.
+// All that depends on nothing but the call's inputs, in one launch: workgroups [0, b0) row pieces, [b0, b1) column
+// partials, [b1, b2) b transposed, [b2, b3) a transposed.  2,048 x 25,088 x 1,024 fp32: 58 us, 0.25 GB at 4.3 TB/s.
 template <typename T, int NV>
 __global__ void __launch_bounds__(256)
 grad_prepare_kernel(const I8Grad A, int b0, int b1, int b2)
@@ -357,7 +364,7 @@ grad_prepare_kernel(const I8Grad A, int b0, int b1, int b2)
     } s;
     int b = blockIdx.x;
     if (b < b0) {
-        gd_row_digits<T, NV>(A, (int64_t)b * 4 + (threadIdx.x >> 6));
+        gd_row_pieces<T, NV>(A, (int64_t)b * 4 + (threadIdx.x >> 6));
     } else if (b < b1) {
         b -= b0;
         const int nx = (A.N + 63) / 64;
@@ -371,13 +378,13 @@ grad_prepare_kernel(const I8Grad A, int b0, int b1, int b2)
     }
 }
 
-// 2,048 x 1,024 fp32 12.7 us, 8,192 x 1,024 bf16 21.9 us: the column's partials, one after the other, are waited for first.
+// 2,048 x 1,024 fp32 14.0 us, 8,192 x 1,024 bf16 24.6 us: the column's partials, one after the other, are waited for first.
 template <typename T>
 __global__ void __launch_bounds__(256)
-grad_col_digits_kernel(const I8Grad A, int n_part)
+grad_col_pieces_kernel(const I8Grad A, int n_part)
 {
-    __shared__ int8_t tile[3][64][68]; // [digit][n][m]
-    __shared__ double inv_s[64];
+    __shared__ __align__(16) _Float16 tile[2][64][68]; // [piece][n][m]
+    __shared__ double ups[64];
     __shared__ uint32_t tops[4][64];
     __shared__ float sums[4][64];
     const T *grad = (const T *)A.grad, *y = (const T *)A.y;
@@ -408,36 +415,35 @@ grad_col_digits_kernel(const I8Grad A, int n_part)
             sum += sums[w][lane];
         }
         const bool finite = top < 0x7f800000u;
-        inv_s[lane] = !finite || top == 0 ? 0.0 : (double)I8_FIX / (double)__uint_as_float(top);
+        ups[lane] = !finite || top == 0 ? 0.0 : i8_pow2(i8_shift(__uint_as_float(top)));
         if (blockIdx.y == 0 && n < N) {
             A.col_top[n] = finite ? __uint_as_float(top) : __builtin_nanf("");
             if (A.grad_bias) A.grad_bias[n] = sum;
         }
     }
     __syncthreads();
-    const double inv = inv_s[lane];
-    float a[16]; // rows 16 wave .. 16 wave + 15 of the tile
+    const double up = ups[lane];
+    double v[16]; // rows 16 wave .. 16 wave + 15 of the tile
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t m = m0 + wave * 16 + i;
-        a[i] = m < A.M && n < N ? gd_grad(grad, y, m * A.grad_stride + n, m * A.y_stride + n) * A.a_scale[m] : 0.0f;
+        v[i] = m < A.M && n < N ? (double)gd_grad(grad, y, m * A.grad_stride + n, m * A.y_stride + n) * (double)A.a_scale[m] : 0.0;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        int q[3][4];
+        I8Vec<_Float16, 4> h[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) i8_digits(inv != 0.0 ? gd_fix(a[4 * i + j], inv) : 0, q[0][j], q[1][j], q[2][j]);
+        for (int j = 0; j < 4; ++j) i8_pieces(up != 0.0 ? v[4 * i + j] * up : 0.0, h[0].v[j], h[1].v[j]);
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
-            *(uint32_t *)&tile[p][lane][wave * 16 + 4 * i] = qr_pack(q[p][0], q[p][1], q[p][2], q[p][3]);
+        for (int p = 0; p < 2; ++p) __builtin_memcpy(__builtin_assume_aligned(&tile[p][lane][wave * 16 + 4 * i], 8), &h[p], 8);
     }
     __syncthreads();
     const int tn = threadIdx.x >> 2, tm = (threadIdx.x & 3) * 16;
     if (n0 + tn >= N || m0 + tm >= A.col_stride) return;
-    for (int p = 0; p < 3; ++p) {
-        uint32_t w[4];
-        for (int j = 0; j < 4; ++j) w[j] = *(const uint32_t *)&tile[p][tn][tm + 4 * j];
-        *(uint4 *)(A.col_digits + ((int64_t)p * N + n0 + tn) * A.col_stride + m0 + tm) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int p = 0; p < 2; ++p) {
+        I8Vec<_Float16, 16> h;
+        __builtin_memcpy(&h, __builtin_assume_aligned(&tile[p][tn][tm], 8), 32);
+        __builtin_memcpy(__builtin_assume_aligned(A.col_pieces + ((int64_t)p * N + n0 + tn) * A.col_stride + m0 + tm, 32), &h, 32);
     }
 }
 
@@ -446,7 +452,7 @@ int frcnn_i8_grad_parts(int M) { return (M + GC_ROWS - 1) / GC_ROWS; }
 template <typename T> static int grad_prepare_t(const I8Grad &A, hipStream_t st)
 {
     const int nx = (A.N + 63) / 64, kx = (A.K + 63) / 64, mx = (A.M + 63) / 64, parts = frcnn_i8_grad_parts(A.M);
-    const int64_t b0 = A.row_digits ? (A.M + 3) / 4 : 0, b1 = b0 + (A.part_top ? (int64_t)nx * parts : 0),
+    const int64_t b0 = A.row_pieces ? (A.M + 3) / 4 : 0, b1 = b0 + (A.part_top ? (int64_t)nx * parts : 0),
                   b2 = b1 + (A.b_t ? (int64_t)kx * nx : 0), b3 = b2 + (A.a_t ? (int64_t)kx * mx : 0);
     if (A.N <= 256)
         hipLaunchKernelGGL((grad_prepare_kernel<T, 1>), dim3((unsigned)b3), dim3(256), 0, st, A, (int)b0, (int)b1, (int)b2);
@@ -454,8 +460,8 @@ template <typename T> static int grad_prepare_t(const I8Grad &A, hipStream_t st)
         hipLaunchKernelGGL((grad_prepare_kernel<T, 4>), dim3((unsigned)b3), dim3(256), 0, st, A, (int)b0, (int)b1, (int)b2);
     FRCNN_CHECK_LAUNCH("grad_prepare");
     if (A.part_top) {
-        hipLaunchKernelGGL((grad_col_digits_kernel<T>), dim3(nx, mx), dim3(256), 0, st, A, parts);
-        FRCNN_CHECK_LAUNCH("grad_col_digits");
+        hipLaunchKernelGGL((grad_col_pieces_kernel<T>), dim3(nx, mx), dim3(256), 0, st, A, parts);
+        FRCNN_CHECK_LAUNCH("grad_col_pieces");
     }
     return FRCNN_OK;
 }

@@ -1150,7 +1150,8 @@ def linear_i8_backward(grad, y, codes, scale, weight_codes, weight_scale, x_dtyp
                        weight_dtype=torch.float32, want=(True, True, True)):
     """Straight-through gradients of matmul_i8 (rounding counts as the identity): grad (M,N) = dL/dout in y's type, y
     the layer's output if it ended in a ReLU, else None.  -> (grad_x (M,K), grad_weight (N,K), grad_bias (N) fp32),
-    None where not wanted.  Exact sums over 24-bit fixed-point gradients: the same bits every run."""
+    None where not wanted.  A factor (gradient times scale) is held to 2^-23 of itself (2^-50 of its row's or column's
+    largest where it lies below 2^-27 of that), the sums are fp32, in a fixed order: the same bits every run."""
     _need_gpu(grad)
     M, K = codes.shape
     N = weight_codes.shape[0]

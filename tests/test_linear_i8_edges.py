@@ -5,7 +5,8 @@ import ctypes
 import pytest
 import torch
 
-from .test_linear_i8 import BF16, F16, F32, dev, features, gpu, grad_bound, plain_codes, plain_grads, plain_product, same_bits  # noqa: F401,E501
+from .test_linear_i8 import BF16, F16, F32, dev, features, gpu, plain_codes, plain_grads, plain_product, same_bits  # noqa: F401
+from .test_linear_i8 import test_gradients_against_the_formulas as _against_the_formulas
 
 
 # ------------------------------------------------------------------------------------------------ sizes past 32 bits
@@ -39,3 +40,61 @@ def test_python_refuses_sizes_past_32_bits(dev):
                 lambda: ops.LinearI8.apply(many, x, None, False), lambda: ops.LinearI8.apply(x, many, None, False)):
         with pytest.raises(ValueError):
             bad()
+
+
+# --------------------------------------------------------------------------- gradients whose factors differ widely in size
+def float_bound(factors, codes, ref, dtype):
+    """factors (R,I), codes (I,C), ref (R,C).  A factor is held to 2^-23 of itself, or 2^-50 of its row's largest; its product
+    with a code is exact; the I products of an output are added in fp32, each addition off by at most one step, 2^-23, of
+    what has been added, which is at most the sum of magnitudes (the second pieces' sum, 2^-10 of that, likewise); the result
+    is rounded to fp32 and to `dtype`, half a step of each, and half of the smallest subnormal number."""
+    inner = codes.shape[0]
+    top = factors.abs().amax(1, keepdim=True)
+    held = (1 + inner * (1 + 2.0 ** -10)) * 2.0 ** -23 * (factors.abs() @ codes.abs()) + 2.0 ** -50 * top * codes.abs().sum(0)
+    sub = {F16: 2.0 ** -25, BF16: 2.0 ** -134}.get(dtype, 0.0) + 2.0 ** -150
+    return held + (torch.finfo(dtype).eps / 2 + 2.0 ** -24) * (ref.abs() + held) + sub
+
+
+def _skewed(kind, m, n, g):
+    if kind == "confident":  # cross-entropy of a classifier that is sure, and mostly right
+        logits = 12 * torch.randn((m, n), generator=g)
+        label = torch.where(torch.rand((m,), generator=g) < 0.98, logits.argmax(1), torch.randint(0, n, (m,), generator=g))
+        logits[torch.arange(m), label] += 12
+        p = torch.softmax(logits, 1)
+        p[torch.arange(m), label] -= 1
+        return p / m
+    grad = 0.05 * torch.randn((m, n), generator=g)
+    if kind == "tiny":  # the factors are subnormal numbers of fp32
+        return grad * 1e-37
+    grad[m // 3] *= kind  # one row far above the others
+    return grad
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["confident", 1e6, 1e9, 1e15, "tiny"])
+@pytest.mark.parametrize("m,n,k,relu", [(2048, 105, 300, False), (130, 37, 64, True), (70, 2500, 65, False), (5003, 33, 130, True)])
+def test_gradients_of_factors_far_apart(dev, m, n, k, relu, kind):
+    """Against the formulas, each output by the magnitudes of its OWN terms: features are sparse, so that many outputs have
+    nothing of the row's or the column's largest factor in them."""
+    from objectdetection_amd import ops
+    g = torch.Generator().manual_seed(m + n)
+    x = features(m, k, 23) * (torch.rand((m, k), generator=g) < 0.1)
+    w = torch.randn((n, k), generator=g) * 0.05 * (torch.rand((n, k), generator=g) < 0.2)
+    grad = _skewed(kind, m, n, g)
+    leaves = [t.to(dev).requires_grad_() for t in (x, w)]
+    y = ops.LinearI8.apply(leaves[0], leaves[1], None, relu)
+    gx, gw = torch.autograd.grad(y, leaves, grad.to(dev))
+    (q, s), (p, t) = plain_codes(x), plain_codes(w)
+    gm, rx, rw, _ = plain_grads(grad, y.detach().cpu() if relu else None, q, s, p, t)
+    fx, fw = gm * t.double(), (gm * s.double()[:, None]).t()
+    for got, f, c, ref in ((gx, fx, p, rx), (gw, fw, q, rw)):
+        bad = (got.cpu().double() - ref).abs() > float_bound(f, c, ref, F32)
+        assert not bad.any(), (int(bad.sum()), bad.numel(), got.cpu()[bad][:3], ref[bad][:3])
+
+
+@gpu
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32)])
+@pytest.mark.parametrize("m,n,k", [(257, 1030, 12545), (2100, 130, 7000)])
+def test_gradients_by_large_tiles(dev, m, n, k, dtype, wdtype):
+    """Products with enough tiles of 128 x 256 to fill the chip, none of their sides a multiple of a tile's."""
+    _against_the_formulas(dev, m, n, k, dtype, wdtype, True)
