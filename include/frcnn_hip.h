@@ -381,7 +381,8 @@ int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_stride, int M, i
 /* out[m,n] = (sum_k a[m,k] b[n,k]) a_scale[m] b_scale[n] + bias[n], then max(., 0) if relu; NaN stays NaN.
  * a: (M,K) bytes, b: (N,K) bytes, row strides in bytes (16-byte aligned rows are read in place, others are copied to
  * the workspace first); K <= 131071: the 32-bit sums cannot wrap, whatever the bytes.  bias: (N) fp32 or NULL.  The
- * sums are exact, scales and bias are applied in 64 bits, and the result is rounded to fp32 and then to out's type.
+ * sums are exact; sum, scales and bias are rounded once to 64 bits (which keeps the exact expression's sign), then to fp32,
+ * then to out's type.
  * n_rows as above: rows of out behind it are left as they were.  out: (M,N), row stride in elements.
  * workspace: frcnn_matmul_i8_workspace_bytes(M,N,K) bytes, 256-byte aligned, contents need not survive. */
 size_t frcnn_matmul_i8_workspace_bytes(int M, int N, int K);

@@ -37,10 +37,11 @@ struct LiArgs {
 // Row length of a split's sums: quads of neighbours are stored whole
 __host__ __device__ __forceinline__ int li_ld4(int N) { return (N + 3) & ~3; }
 
-// One result from an exact sum: the scales and the bias in 64 bits, then fp32.
+// One result from an exact sum: the scales' product is exact in 64 bits (24 bits each; sum times scale would take up to 55), so
+// that sum, scales and bias are rounded once, to 64 bits, and keep the exact expression's sign; then fp32.
 __device__ __forceinline__ float li_finish(double sum, double a_scale, double b_scale, double bias, int relu)
 {
-    const float z = (float)__builtin_fma(sum * a_scale, b_scale, bias);
+    const float z = (float)__builtin_fma(sum, a_scale * b_scale, bias);
     return relu && z < 0.0f ? 0.0f : z; // keeps NaN
 }
 

@@ -98,3 +98,40 @@ def test_gradients_of_factors_far_apart(dev, m, n, k, relu, kind):
 def test_gradients_by_large_tiles(dev, m, n, k, dtype, wdtype):
     """Products with enough tiles of 128 x 256 to fill the chip, none of their sides a multiple of a tile's."""
     _against_the_formulas(dev, m, n, k, dtype, wdtype, True)
+
+
+# ------------------------------------------------------------------------------------ signs that hang on the last bit
+def _row_with_sum(total, k):
+    """Bytes a, b (k) with sum a b = total (>= 0)."""
+    a, b = torch.zeros(k, dtype=torch.int64), torch.zeros(k, dtype=torch.int64)
+    full, rest = divmod(total, 127 * 127)
+    assert full + 2 <= k
+    a[:full] = b[:full] = 127
+    a[full], b[full] = 127, rest // 127
+    a[full + 1], b[full + 1] = 1, rest % 127
+    assert int((a * b).sum()) == total
+    return a.to(torch.int8), b.to(torch.int8)
+
+
+@gpu
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("m", [2, 40])
+def test_sign_of_a_sum_that_53_bits_do_not_hold(dev, m, sign):
+    """sum * a_scale needs 55 bits and the bias cancels all but its last: what is left is one unit, to which the ReLU's sign
+    and the result's value both hang."""
+    from objectdetection_amd import ops
+    k = 131071
+    scale = next(v for v in range((1 << 24) - 1, 1 << 23, -2)  # an odd 24-bit number, times its inverse modulo 2^31
+                 if 2060000000 < pow(v, -1, 1 << 31) * sign % (1 << 31) < 2110000000)
+    total = pow(scale, -1, 1 << 31) * sign % (1 << 31)
+    left = total * scale - sign
+    assert left % (1 << 31) == 0 and left >> 31 < 1 << 24 and (total * scale).bit_length() == 55
+    a, b = _row_with_sum(total, k)
+    codes = a.repeat(m, 1).to(dev)
+    unit = 2.0 ** -20
+    out = ops.matmul_i8(codes, torch.full((m,), float(scale), device=dev), b[None].to(dev), torch.tensor([unit], device=dev),
+                        torch.tensor([-float(left) * unit], device=dev), False)
+    assert (out == sign * unit).all(), out[:2]
+    out = ops.matmul_i8(codes, torch.full((m,), float(scale), device=dev), b[None].to(dev), torch.tensor([unit], device=dev),
+                        torch.tensor([-float(left) * unit], device=dev), True)
+    assert (out == max(sign, 0) * unit).all(), out[:2]
