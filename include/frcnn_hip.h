@@ -382,7 +382,8 @@ int frcnn_quantize_rows_i8(const void *x, int x_type, int64_t x_stride, int M, i
  * a: (M,K) bytes, b: (N,K) bytes, row strides in bytes (16-byte aligned rows are read in place, others are copied to
  * the workspace first); K <= 131071: the 32-bit sums cannot wrap, whatever the bytes.  bias: (N) fp32 or NULL.  The
  * sums are exact; sum, scales and bias are rounded once to 64 bits (which keeps the exact expression's sign), then to fp32,
- * then to out's type.
+ * then to out's type.  With relu a positive result that out's type rounds to zero is stored as -0, what the ReLU cut off as
+ * +0: the backward call below tells them apart.
  * n_rows as above: rows of out behind it are left as they were.  out: (M,N), row stride in elements.
  * workspace: frcnn_matmul_i8_workspace_bytes(M,N,K) bytes, 256-byte aligned, contents need not survive. */
 size_t frcnn_matmul_i8_workspace_bytes(int M, int N, int K);
@@ -412,8 +413,8 @@ int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride, const voi
                           size_t workspace_bytes, void *stream);
 
 /* Straight-through gradients of the layer (rounding counts as the identity), from grad = dL/dout (M,N) and the codes
- * and scales of the forward call.  g = grad, or 0 where y <= 0 (y: the forward's output in grad's type if it ended in
- * a ReLU, NULL otherwise):
+ * and scales of the forward call.  g = grad, or 0 where y is below zero or +0 (y: the forward's output in grad's type if it
+ * ended in a ReLU, NULL otherwise; -0 is a positive result, see above):
  *   grad_x[m,k] = sum_n g[m,n] b_scale[n] b[n,k]     grad_w[n,k] = sum_m g[m,n] a_scale[m] a[m,k]
  *   grad_bias[n] = sum_m g[m,n]  (fp32, summed in a fixed order)
  * Each factor g b_scale and g a_scale is held to 2^-23 of itself, or to 2^-50 of the largest of its row m (grad_x) or

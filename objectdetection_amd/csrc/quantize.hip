@@ -206,12 +206,13 @@ int frcnn_i8_pad_rows(const int8_t *src, int64_t src_stride, int rows, int K, in
 }
 
 // ---- what the gradients' products are made from ----------------------------------------------------------------------
-// g_mn = grad_mn, or 0 where a ReLU's output y_mn is not above 0 (y = NULL: no ReLU; a NaN lets the gradient through, as
-// torch's threshold backward does).
+// g_mn = grad_mn, or 0 where a ReLU cut: where its output y_mn is below zero or +0 (y = NULL: no ReLU).  -0 stands for a
+// positive number that the output's type rounds to zero; a NaN lets the gradient through, as torch's threshold backward does.
+__device__ __forceinline__ bool gd_cut(float y) { return y <= 0.0f && __float_as_uint(y) != 0x80000000u; }
 template <typename T> __device__ __forceinline__ float gd_grad(const T *grad, const T *y, int64_t gi, int64_t yi)
 {
     const float g = (float)grad[gi];
-    return y && (float)y[yi] <= 0.0f ? 0.0f : g;
+    return y && gd_cut((float)y[yi]) ? 0.0f : g;
 }
 
 // Codes (rows, cols) -> fp16 (cols, rows), one 64 x 64 tile; a thread reads 16 codes of a row and writes 16 of a column.
@@ -259,7 +260,7 @@ __device__ __forceinline__ void gd_row_pieces(const I8Grad &A, int64_t row)
             if (z) u = i8_load<T, 4>(z + n);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                a.g[j] = z && (float)u.v[j] <= 0.0f ? 0.0f : (float)v.v[j];
+                a.g[j] = z && gd_cut((float)u.v[j]) ? 0.0f : (float)v.v[j];
                 a.s[j] = c.v[j];
             }
         } else {

@@ -1103,7 +1103,8 @@ def quantize_rows_i8(x, n_rows=None):
 
 def matmul_i8(codes, scale, weight_codes, weight_scale, bias=None, relu=False, out_dtype=torch.float32, n_rows=None):
     """out (M,N) = (codes @ weight_codes^T) * scale[:, None] * weight_scale + bias, then max(., 0) if relu: the product
-    of two row-quantised matrices (quantize_rows_i8), its sums exact, the rest in 64 bits, rounded to out_dtype."""
+    of two row-quantised matrices (quantize_rows_i8), its sums exact, the rest in 64 bits, rounded to out_dtype.  With relu
+    a positive result that out_dtype rounds to zero is -0.0, which is how linear_i8_backward knows it."""
     _need_gpu(codes, scale)
     if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] == 0 or scale.shape != (codes.shape[0],):
         raise ValueError("matmul_i8 expects codes (M,K) int8 and a scale for each row; got %s %s, %s"
@@ -1149,7 +1150,7 @@ def linear_i8(x, weight_codes, weight_scale, bias=None, relu=False, out_dtype=No
 def linear_i8_backward(grad, y, codes, scale, weight_codes, weight_scale, x_dtype=torch.float32,
                        weight_dtype=torch.float32, want=(True, True, True)):
     """Straight-through gradients of matmul_i8 (rounding counts as the identity): grad (M,N) = dL/dout in y's type, y
-    the layer's output if it ended in a ReLU, else None.  -> (grad_x (M,K), grad_weight (N,K), grad_bias (N) fp32),
+    the layer's output if it ended in a ReLU (its gradient passes where y > 0 or y is -0.0), else None.  -> (grad_x (M,K), grad_weight (N,K), grad_bias (N) fp32),
     None where not wanted.  A factor (gradient times scale) is held to 2^-23 of itself (2^-50 of its row's or column's
     largest where it lies below 2^-27 of that), the sums are fp32, in a fixed order: the same bits every run."""
     _need_gpu(grad)

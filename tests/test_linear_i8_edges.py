@@ -135,3 +135,39 @@ def test_sign_of_a_sum_that_53_bits_do_not_hold(dev, m, sign):
     out = ops.matmul_i8(codes, torch.full((m,), float(scale), device=dev), b[None].to(dev), torch.tensor([unit], device=dev),
                         torch.tensor([-float(left) * unit], device=dev), True)
     assert (out == max(sign, 0) * unit).all(), out[:2]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 100), (60, 70, 300), (99, 64, 4100), (600, 520, 1100), (40, 33, 33001)])
+def test_relu_lets_gradients_through_where_the_sum_is_positive(dev, m, n, k, dtype):
+    """Outputs around the border where their type rounds to zero: the gate is the sum's sign, not the rounded output's.  The
+    output itself stays the rounded one."""
+    from objectdetection_amd import ops
+    g = torch.Generator().manual_seed(k)
+    low = {F32: 2.0 ** -150, BF16: 2.0 ** -134, F16: 2.0 ** -25}[dtype]  # rounds to zero, and what is above does not
+    x = features(m, k, 31, torch.float64) * (2.0 ** -70 if dtype != F16 else 1.0)
+    x = x.to(dtype)
+    w = torch.randn((n, k), generator=g)
+    w *= low / float((x.double() @ w.double().t()).abs().median())
+    grad = torch.randn((m, n), generator=g).to(dtype)
+    leaves = [t.to(dev).requires_grad_() for t in (x, w, torch.zeros(n))]
+    y = ops.LinearI8.apply(*leaves, True)
+    gx, gw, gb = torch.autograd.grad(y, leaves, grad.to(dev))
+    (q, s), (p, t) = plain_codes(x), plain_codes(w)
+    same_bits(y, plain_product(q, s, p, t, None, True, dtype))
+    z = (q @ p.t()) * s.double()[:, None] * t.double()
+    assert ((z > 0) & (y.cpu() == 0)).sum() > m * n / 20 and (y > 0).sum() > m * n / 20
+    gm = torch.where(z > 0, grad.double(), torch.zeros_like(z))
+    fx, fw = gm * t.double(), (gm * s.double()[:, None]).t()
+    rx, rw = fx @ p, fw @ q
+    assert ((gx.cpu().double() - rx).abs() <= float_bound(fx, p, rx, dtype)).all()
+    assert ((gw.cpu().double() - rw).abs() <= float_bound(fw, q, rw, F32)).all()
+    assert ((gb.cpu().double() - gm.sum(0)).abs() <= (m + 1) * 2.0 ** -24 * gm.abs().sum(0) + 1e-45).all()
+    # the same from the single calls
+    c, a = ops.quantize_rows_i8(leaves[0])
+    wc, b = ops.quantize_rows_i8(leaves[1])
+    z = ops.matmul_i8(c, a, wc, b, leaves[2], True, dtype)
+    same_bits(z, y)
+    for u, v in zip(ops.linear_i8_backward(grad.to(dev), z, c, a, wc, b, dtype, F32), (gx, gw, gb)):
+        same_bits(u, v)
