@@ -7,9 +7,42 @@ device-side row count, keeps the rows behind it out without a host read.  To tra
 the float modules with int8=True.
 """
 import torch
-from torch.nn import Module
+from torch.nn import Linear, Module, functional
+from torch.nn.modules import module as _module
 
 from .. import ops
+
+
+class Int8TrainingLinear(Linear):
+    """torch's Linear with its product on 8-bit integers, differentiable (ops.LinearI8): what TwoMLPHead and
+    FasterRCNNPredictor are made of with int8=True.  Same parameters and state_dict.  Takes (M,K)."""
+
+    def forward(self, x):
+        return ops.LinearI8.apply(x, self.weight, self.bias, False)
+
+
+def follow(layers, int8):
+    """A head's own layers take the class of its choice, which may come later than they (set on a finished module, or one
+    pickled before it): the two classes hold the same."""
+    for layer in layers:
+        if type(layer) is (Linear if int8 else Int8TrainingLinear):
+            layer.__class__ = Int8TrainingLinear if int8 else Linear
+
+
+def fuses(layer):
+    """Whether a caller may compute this layer together with what follows: not where someone watches or changes what goes in
+    and out (hooks; weight normalisation as a pre-hook is one), nor a layer put in its place."""
+    return isinstance(layer, Int8TrainingLinear) and not (
+        layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks or layer._backward_pre_hooks
+        or _module._global_forward_hooks or _module._global_forward_pre_hooks or _module._global_backward_hooks
+        or _module._global_backward_pre_hooks)
+
+
+def dense_relu(layer, x):
+    """relu(layer(x)), in one call where nothing needs the layer's own output."""
+    if fuses(layer):
+        return ops.LinearI8.apply(x, layer.weight, layer.bias, True)
+    return functional.relu(layer(x))
 
 
 class Int8Linear(Module):

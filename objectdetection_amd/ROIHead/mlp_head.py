@@ -2,7 +2,7 @@
 train with straight-through gradients (ops.LinearI8); Int8TwoMLPHead serves what either has learnt."""
 from torch.nn import Linear, Module, functional
 
-from .. import ops
+from .int8 import Int8TrainingLinear, dense_relu, follow
 
 
 class TwoMLPHead(Module):
@@ -10,15 +10,16 @@ class TwoMLPHead(Module):
 
     def __init__(self, in_channels, representation_size, int8=False):
         super().__init__()
-        self.fc1 = Linear(in_channels, representation_size)
-        self.fc2 = Linear(representation_size, representation_size)
+        layer = Int8TrainingLinear if int8 else Linear
+        self.fc1 = layer(in_channels, representation_size)
+        self.fc2 = layer(representation_size, representation_size)
         self.int8 = int8
 
     def forward(self, x):
         x = x.flatten(start_dim=1)
+        follow((self.fc1, self.fc2), self.int8)
         if self.int8:
-            x = ops.LinearI8.apply(x, self.fc1.weight, self.fc1.bias, True)
-            return ops.LinearI8.apply(x, self.fc2.weight, self.fc2.bias, True)
+            return dense_relu(self.fc2, dense_relu(self.fc1, x))
         x = functional.relu(self.fc1(x))
         x = functional.relu(self.fc2(x))
         return x

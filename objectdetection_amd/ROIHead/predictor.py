@@ -5,6 +5,7 @@ import torch
 from torch.nn import Linear, Module
 
 from .. import ops
+from .int8 import Int8TrainingLinear, follow, fuses
 
 
 class FasterRCNNPredictor(Module):
@@ -12,13 +13,16 @@ class FasterRCNNPredictor(Module):
 
     def __init__(self, in_channels, num_classes, int8=False):
         super().__init__()
-        self.cls_score = Linear(in_channels, num_classes)
-        self.bbox_pred = Linear(in_channels, num_classes * 4)
+        layer = Int8TrainingLinear if int8 else Linear
+        self.cls_score = layer(in_channels, num_classes)
+        self.bbox_pred = layer(in_channels, num_classes * 4)
         self.int8 = int8
 
     def forward(self, x):
         x = x.flatten(start_dim=1)
-        if self.int8:  # one product: x is quantised once
+        follow((self.cls_score, self.bbox_pred), self.int8)
+        if self.int8 and fuses(self.cls_score) and fuses(self.bbox_pred) and self.cls_score.bias is not None \
+                and self.bbox_pred.bias is not None:  # one product: x is quantised once
             y = ops.LinearI8.apply(x, torch.cat([self.cls_score.weight, self.bbox_pred.weight]),
                                    torch.cat([self.cls_score.bias, self.bbox_pred.bias]), False)
             return y[:, :self.cls_score.out_features], y[:, self.cls_score.out_features:]
