@@ -420,7 +420,8 @@ int frcnn_linear_i8_train(const void *x, int x_type, int64_t x_stride, const voi
  * Each factor g b_scale and g a_scale is held to 2^-23 of itself, or to 2^-50 of the largest of its row m (grad_x) or
  * column n (grad_w), whichever is more; its product with a code is exact and the sums are fp32, so an output is off by what
  * an fp32 product of the same factors is.  An Inf or a NaN among a row's (column's) factors makes that whole
- * row of grad_x (grad_w) NaN.  grad_x / grad_w: contiguous; grad_x, grad_w, grad_bias: NULL where not wanted.
+ * row of grad_x (grad_w) NaN.  grad_x / grad_w: contiguous; grad_x, grad_w, grad_bias: NULL where not wanted; a and a_scale
+ * may be NULL where grad_x alone is.
  * M, N, K <= 131071.  The results have the same bits every run. */
 size_t frcnn_linear_i8_backward_workspace_bytes(int M, int N, int K);
 int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t grad_stride, const void *y, int64_t y_stride,

@@ -47,7 +47,8 @@ def dense_relu(layer, x):
 
 class Int8Linear(Module):
     """y = [relu](x W^T + b) with W as codes (N,K) int8 and scales (N) fp32.  Nothing here is trained: weights change only
-    by from_float or load_state_dict, and in training mode an x that wants a gradient is refused."""
+    by from_float or load_state_dict.  In eval mode an x that wants a gradient gets it (straight-through), in training mode
+    it is refused, lest a head that cannot learn goes unnoticed."""
 
     def __init__(self, in_features, out_features, bias=True, relu=False):
         super().__init__()
@@ -80,9 +81,12 @@ class Int8Linear(Module):
         return self
 
     def forward(self, x, n_rows=None, out_dtype=None):
-        if self.training and torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("Int8Linear has no gradient: call eval(), or train TwoMLPHead / FasterRCNNPredictor "
-                               "with int8=True")
+        if torch.is_grad_enabled() and x.requires_grad:
+            if self.training:
+                raise RuntimeError("Int8Linear's weights have no gradient: call eval(), or train TwoMLPHead / "
+                                   "FasterRCNNPredictor with int8=True")
+            return ops.FrozenLinearI8.apply(x, self.codes[:, :self.in_features], self.scale, self.bias, self.relu, out_dtype,
+                                            n_rows)
         return ops.linear_i8(x, self.codes[:, :self.in_features], self.scale, self.bias, self.relu, out_dtype, n_rows)
 
 

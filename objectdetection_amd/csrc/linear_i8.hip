@@ -1096,7 +1096,7 @@ extern "C" int frcnn_linear_i8_backward(const void *grad, int grad_type, int64_t
                   "linear_i8_backward: bad shape (%d, %d, %d); each is at most %d", M, N, K, I8_MAX_K);
     FRCNN_REQUIRE(i8_type_ok(grad_type) && i8_type_ok(grad_x_type) && i8_type_ok(grad_w_type),
                   "linear_i8_backward: unknown element type");
-    FRCNN_REQUIRE(grad && a && a_scale && b && b_scale, "linear_i8_backward: null pointer");
+    FRCNN_REQUIRE(grad && b && b_scale && ((a && a_scale) || (!grad_w && !grad_bias)), "linear_i8_backward: null pointer");
     FRCNN_REQUIRE(grad_stride >= 0 && y_stride >= 0 && a_stride >= 0 && b_stride >= 0, "linear_i8_backward: bad strides");
     const LiGrad l = li_grad(M, N, K);
     FRCNN_REQUIRE(li_ws_ok(workspace), "linear_i8_backward: the workspace has to be 256-byte aligned");

@@ -1128,8 +1128,8 @@ def matmul_i8(codes, scale, weight_codes, weight_scale, bias=None, relu=False, o
 def linear_i8(x, weight_codes, weight_scale, bias=None, relu=False, out_dtype=None, n_rows=None):
     """A served dense layer: quantize_rows_i8(x) and matmul_i8 in one call.  x (M,K) fp32, bf16 or fp16; weight_codes
     (N,K) int8 and weight_scale (N) from quantize_rows_i8(weight); -> (M,N) in out_dtype (x's type by default).
-    n_rows (1) int32 on the device: rows behind it are neither read nor written.  The result is detached; LinearI8 is
-    the differentiable form."""
+    n_rows (1) int32 on the device: rows behind it are neither read nor written.  The result is detached; FrozenLinearI8
+    also has the gradient of x, LinearI8 trains the weights."""
     x = _i8_rows(x, "linear_i8")
     M, K = x.shape
     dev = x.device
@@ -1187,6 +1187,37 @@ def _i8_backward(grad, y, codes, codes_stride, scale, weight_codes, weight_strid
              weight_scale, M, N, K, _at(gx), _I8_TYPES[x_dtype], _at(gw), _I8_TYPES[weight_dtype], _at(gb),
              ws_at, nbytes)
     return gx, gw, gb
+
+
+class FrozenLinearI8(torch.autograd.Function):
+    """linear_i8 with the gradient of x (the layer's weights have none): apply(x, weight_codes, weight_scale, bias, relu,
+    out_dtype, n_rows).  Rounding of x counts as the identity; rows behind n_rows get zeros."""
+
+    @staticmethod
+    def forward(ctx, x, weight_codes, weight_scale, bias=None, relu=False, out_dtype=None, n_rows=None):
+        y = linear_i8(x, weight_codes, weight_scale, bias, relu, out_dtype, n_rows)
+        ctx.x_dtype = x.dtype
+        ctx.save_for_backward(weight_codes, weight_scale, y if relu else None, n_rows)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        codes, scale, y, n_rows = ctx.saved_tensors
+        M, (N, K) = grad.shape[0], codes.shape
+        if N > I8_MAX_K:
+            raise ValueError("FrozenLinearI8: a gradient of %d channels; at most %d" % (N, I8_MAX_K))
+        if n_rows is not None:
+            grad = grad.where(torch.arange(M, device=grad.device)[:, None] < n_rows, 0)
+        codes, scale = _i8_codes(codes), _f32v(scale)
+        x_dtype = ctx.x_dtype if ctx.x_dtype in _I8_TYPES else torch.float32
+        parts = [grad.new_empty((0, K), dtype=x_dtype)] if M == 0 else []
+        for m in range(0, M, I8_MAX_K):  # a row's gradient is its own: as many rows a call as it takes
+            g, z = grad[m:m + I8_MAX_K], y[m:m + I8_MAX_K] if y is not None else None
+            parts.append(_i8_backward(g, z, None, 0, None, codes.data_ptr(), _row_stride(codes), scale.data_ptr(),
+                                      g.shape[0], N, K, x_dtype, torch.float32, (True, False, False))[0])
+        gx = parts[0] if len(parts) == 1 else torch.cat(parts)
+        return (gx.to(ctx.x_dtype),) + (None,) * 6
 
 
 @functools.lru_cache(maxsize=1024)
