@@ -1068,6 +1068,8 @@ def _i8_count(n_rows, what, dev):
     _i8_device(what, dev, n_rows)
     if n_rows.numel() != 1:
         raise ValueError("%s: n_rows expects one element; got %s" % (what, tuple(n_rows.shape)))
+    if n_rows.dtype in (torch.int64, torch.float32, torch.float64):
+        n_rows = n_rows.clamp(0, I8_MAX_ROWS)  # to within 32 bits, not to their low half
     return n_rows if n_rows.dtype == torch.int32 else n_rows.to(torch.int32)
 
 

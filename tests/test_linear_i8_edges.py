@@ -351,3 +351,15 @@ def test_backward_entry_takes_no_codes_of_x_for_its_gradient_alone():
     for wanted in ((p, p, null), (p, null, p), (null, p, null), (null, null, p)):
         assert bw(*wanted) == -1 and b"null" in lib.frcnn_last_error_string()
     assert bw(p, null, null) == -2 and b"workspace" in lib.frcnn_last_error_string()
+
+
+@gpu
+@pytest.mark.parametrize("count,rows", [((1 << 32) + 3, 20), (-(1 << 32) + 5, 0), (1 << 62, 20), (7, 7), (-1, 0), (2.0 ** 40, 20)])
+def test_counts_past_32_bits(dev, count, rows):
+    """A row count of 64 bits is clamped to the rows that there are, like one of 32."""
+    from objectdetection_amd import ops
+    x = features(20, 70, 8).to(dev)
+    wc, ws = ops.quantize_rows_i8(torch.randn((6, 70), generator=torch.Generator().manual_seed(1)).to(dev))
+    assert int(ops._i8_count(torch.tensor([count], device=dev), "count", dev).clamp(max=20)) == rows
+    out = ops.linear_i8(x, wc, ws, n_rows=torch.tensor([count], device=dev))
+    same_bits(out[:rows], ops.linear_i8(x, wc, ws)[:rows])
