@@ -363,3 +363,46 @@ def test_counts_past_32_bits(dev, count, rows):
     assert int(ops._i8_count(torch.tensor([count], device=dev), "count", dev).clamp(max=20)) == rows
     out = ops.linear_i8(x, wc, ws, n_rows=torch.tensor([count], device=dev))
     same_bits(out[:rows], ops.linear_i8(x, wc, ws)[:rows])
+
+
+# ------------------------------------------------------------------------- training and quantising rows of every length
+@gpu
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("dtype,wdtype", [(F32, F32), (BF16, F32), (F32, F16), (F16, F16)])
+@pytest.mark.parametrize("m,n,k", [(300, 130, 12545), (520, 260, 25088), (40, 70, 33001), (20, 70, 70001), (1100, 40, 2049)])
+def test_training_of_long_rows(dev, m, n, k, dtype, wdtype, relu):
+    """Sums of the forward call split over workgroups and joined, both operands quantised by the forms for long rows (in one
+    launch, in two where their types differ, by two passes), gradients over many tiles of k."""
+    _against_the_formulas(dev, m, n, k, dtype, wdtype, relu)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [65537, 70003, 131072])
+def test_quantize_rows_in_two_passes(dev, k, dtype):
+    """Rows too long for the registers in every type: the ends of the type, a row of zeros, Inf and NaN in the last element, an
+    odd offset, codes on an odd stride, a row behind the count."""
+    from objectdetection_amd import _lib, ops
+    fin = torch.finfo(dtype)
+    base = features(8, k + 3, k, torch.float64)
+    base[:, k] = 1.0
+    for i, top in enumerate((fin.max, fin.tiny, fin.tiny * fin.eps * 5, 0.0)):
+        base[i] *= top / base[i].abs().max()
+    base = base.to(dtype)
+    base[4, k], base[5, k] = float("inf"), float("nan")
+    base[6, 2::3] *= -1
+    ref, ref_scale = plain_codes(base[:, 1:k + 1])
+    on = base.to(dev)[:, 1:k + 1]
+    codes, scale = ops.quantize_rows_i8(on)
+    assert torch.equal(codes.cpu().double(), ref)
+    same_bits(scale, ref_scale)
+    odd = torch.full((8, k + 2 - k % 2 + 1), 77, dtype=torch.int8, device=dev)
+    scale = torch.full((8,), 5.0, device=dev)
+    P = ctypes.c_void_p
+    n = torch.tensor([7], dtype=torch.int32, device=dev)
+    assert _lib.load().frcnn_quantize_rows_i8(P(on.data_ptr()), ops._I8_TYPES[dtype], on.stride(0), 8, k, P(n.data_ptr()),
+                                              P(odd.data_ptr()), odd.stride(0), P(scale.data_ptr()),
+                                              P(torch.cuda.current_stream().cuda_stream)) == 0
+    assert torch.equal(odd.cpu()[:7, :k].double(), ref[:7]) and (odd[:, k:] == 77).all() and (odd[7] == 77).all()
+    same_bits(scale[:7], ref_scale[:7])
+    assert scale[7] == 5
