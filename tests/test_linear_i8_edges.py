@@ -406,3 +406,78 @@ def test_quantize_rows_in_two_passes(dev, k, dtype):
     assert torch.equal(odd.cpu()[:7, :k].double(), ref[:7]) and (odd[:, k:] == 77).all() and (odd[7] == 77).all()
     same_bits(scale[:7], ref_scale[:7])
     assert scale[7] == 5
+
+
+# --------------------------------------------------------------------------------------------------- captured and side by side
+@gpu
+@pytest.mark.parametrize("m,n,k", [(300, 130, 12545), (257, 1030, 12545)])
+def test_captured_training_of_long_rows(dev, m, n, k):
+    """Forward and backward with split sums and by large tiles, and the served layer's gradient behind a row count, in one
+    graph; replayed on new inputs with eager work between, each against the eager result; another graph's workspaces beside
+    it."""
+    from objectdetection_amd import ops
+    g = torch.Generator().manual_seed(m)
+    x = features(m, k, 41).to(dev).requires_grad_()
+    w = (0.05 * torch.randn((n, k), generator=g)).to(dev).requires_grad_()
+    b = torch.randn((n,), generator=g).to(dev).requires_grad_()
+    up = torch.randn((m, n), generator=g).to(dev)
+    wc, ws = ops.quantize_rows_i8(w)
+    count = torch.tensor([m - 7], dtype=torch.int32, device=dev)
+
+    def train():
+        y = ops.LinearI8.apply(x, w, b, True)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b), up)
+
+    def serve():
+        y = ops.FrozenLinearI8.apply(x, wc, ws, b.detach(), True, None, count)
+        # rows of the output behind the smallest count, m - 51, are unspecified; those of the gradient are zeros
+        return y.detach()[:m - 51], torch.autograd.grad(y, x, up)[0]
+    side = torch.cuda.Stream(device=dev)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train(), serve()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for step in (train, serve):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        graphs.append((graph, held, step))
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(features(m, k, 50 + i).to(dev))
+            w.mul_(-0.5)
+            up.neg_()
+            count.sub_(11)
+        for graph, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, held, step in graphs:
+            got = [t.clone() for t in held]
+            for u, v in zip(got, step()):
+                same_bits(u, v)
+
+
+@gpu
+def test_training_on_two_streams(dev):
+    """Two training steps at once on streams of their own, with inputs of their own."""
+    from objectdetection_amd import ops
+    steps, eager, got = [], [], [[], []]
+    for i in range(2):
+        leaves = [features(300, 12545, 60 + i).to(dev).requires_grad_(),
+                  torch.randn((130, 12545), generator=torch.Generator().manual_seed(i)).to(dev).requires_grad_()]
+        steps.append(lambda leaves=leaves: torch.autograd.grad(ops.LinearI8.apply(*leaves, None, True).square().sum(), leaves))
+        eager.append(steps[i]())
+    streams = [torch.cuda.Stream(device=dev) for _ in steps]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(steps[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        for grads in got[i]:
+            for u, v in zip(grads, eager[i]):
+                same_bits(u, v)
