@@ -25,8 +25,8 @@ struct LiArgs {
     int M, N, K;                         // K: bytes of a row's k (two pieces: two a number, zeros up to a multiple of 32)
     int tiles_m, tiles_n, k_split;       // k_split: bytes of k per split, a multiple of LI_BK
     const float *a_scale, *b_scale, *bias;
-    int relu, out_type;
-    float low;                           // the largest fp32 number that out's type rounds to zero
+    int out_type;
+    float low;                           // ReLU: the largest fp32 number that out's type rounds to zero; none: NaN
     bool stream;                         // results stored past the caches
     void *out;
     int64_t out_stride;                  // elements
@@ -41,12 +41,15 @@ __host__ __device__ __forceinline__ int li_ld4(int N) { return (N + 3) & ~3; }
 // One result from an exact sum: the scales' product is exact in 64 bits (24 bits each; sum times scale would take up to 55), so
 // that sum, scales and bias are rounded once, to 64 bits, and keep the exact expression's sign; then fp32.
 // Behind a ReLU a zero tells what it was: -0 for a positive result that the output's type rounds to zero (`low`: the largest
-// number that it does), +0 for what the ReLU cut off.  Both are equal to zero; the backward call reads the difference.
-__device__ __forceinline__ float li_finish(double sum, double a_scale, double b_scale, double bias, int relu, float low)
+// number that it does; NaN without a ReLU, so that one comparison decides), +0 for what the ReLU cut off.  Both are equal to
+// zero; the backward call reads the difference.
+__device__ __forceinline__ float li_finish(double sum, double a_scale, double b_scale, double bias, float low)
 {
     const double zd = __builtin_fma(sum, a_scale * b_scale, bias);
     const float z = (float)zd;
-    return !relu || !(z <= low) ? z : (zd > 0.0 ? -0.0f : 0.0f); // keeps NaN
+    // zd > 0 by its upper half: fp32 scales and biases leave nothing between 0 and 2^-1022
+    const float zero = __double2hiint(zd) > 0 ? -0.0f : 0.0f;
+    return z <= low ? zero : z; // keeps NaN
 }
 
 // P: planes of a.  1: bytes, whole-number sums.  2: the pieces of a gradient's factor, fp32 sums.
@@ -311,7 +314,7 @@ __device__ __forceinline__ void linear_i8_tile(const LiArgs &A, int block, int s
                 const int m = mw + tm * 16;
                 float z[V];
 #pragma unroll
-                for (int r = 0; r < V; ++r) z[r] = li_finish(sum(tm, tn + r / 4, r % 4), sa[tm], sb[r], bias[r], A.relu, A.low);
+                for (int r = 0; r < V; ++r) z[r] = li_finish(sum(tm, tn + r / 4, r % 4), sa[tm], sb[r], bias[r], A.low);
                 if (m < M) li_store<decltype(stream)::value>(out + (int64_t)m * A.out_stride + n, z, A.N - n);
             }
         }
@@ -379,7 +382,7 @@ template <int P> __device__ __forceinline__ void linear_i8_join(const LiArgs &A,
     for (int r = 0; r < 4; ++r) {
         const int nr = n + r < A.N ? n + r : A.N - 1;
         z[r] = li_finish((double)t[r], a_scale, P == 1 ? (double)A.b_scale[nr] : 1.0,
-                         P == 1 && A.bias ? (double)A.bias[nr] : 0.0, A.relu, A.low);
+                         P == 1 && A.bias ? (double)A.bias[nr] : 0.0, A.low);
     }
     const int64_t at = (int64_t)m * A.out_stride + n;
     if (A.out_type == FRCNN_F32) li_store((float *)A.out + at, z, A.N - n);
@@ -498,7 +501,7 @@ linear_i8_few_kernel(const T *__restrict__ x, int64_t x_stride, const float *__r
             int total = 0;
             for (int v = 0; v < LF_THREADS / 64; ++v) total += sums[v][t];
             const int n = n0 + t;
-            const float z = li_finish((double)total, (double)scale, (double)A.b_scale[n], A.bias ? (double)A.bias[n] : 0.0, A.relu, A.low);
+            const float z = li_finish((double)total, (double)scale, (double)A.b_scale[n], A.bias ? (double)A.bias[n] : 0.0, A.low);
             li_store_as(A, m * A.out_stride + n, z);
         }
         __syncthreads(); // red and sums are the next row's
@@ -662,7 +665,7 @@ __device__ __forceinline__ void linear_i8_short(const T *__restrict__ x, int64_t
                 const int m = m0 + tm * 16 + i16;
                 float z[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[r] = li_finish((double)acc[tm][r], sa[tm], sb[r], bias[r], A.relu, A.low);
+                for (int r = 0; r < 4; ++r) z[r] = li_finish((double)acc[tm][r], sa[tm], sb[r], bias[r], A.low);
                 if (m < M) li_store(out + (int64_t)m * A.out_stride + n, z, n_end - n);
             }
         };
@@ -894,10 +897,10 @@ static LiArgs li_args(const int8_t *a, int64_t a_stride, const float *a_scale, c
     LiArgs A = {};
     A.a = a; A.a_stride = a_stride; A.a_scale = a_scale;
     A.b = b; A.b_stride = b_stride; A.b_scale = b_scale;
-    A.bias = bias; A.relu = relu;
+    A.bias = bias;
     A.M = M; A.N = N; A.K = K; A.n_rows = n_rows;
     A.out = out; A.out_type = out_type; A.out_stride = out_stride;
-    A.low = out_type == FRCNN_F16 ? 0x1p-25f : out_type == FRCNN_BF16 ? 0x1p-134f : 0.0f;
+    A.low = !relu ? __builtin_nanf("") : out_type == FRCNN_F16 ? 0x1p-25f : out_type == FRCNN_BF16 ? 0x1p-134f : 0.0f;
     A.stream = (((uintptr_t)out | (uint64_t)out_stride * i8_type_bytes(out_type)) & 63) == 0;
     return A;
 }
