@@ -117,9 +117,9 @@ __device__ __forceinline__ void li_tile(int block, int tiles_m, int tiles_n, int
     tn = rem / gm;
 }
 
-// Many rows of a product are bound by the clock under load: 32,000 x 25,088 x 1,024 by 256 x 256 tiles takes 684 us,
-// 2.40 POPS, with the matrix pipes busy in 55 % of the cycles at 2.05 GHz (zeros for operands and no traffic: 447 us where
-// this took 712).  At k = 1,024 (to bf16, 45 us) the stores and the 64-bit epilogue, which nothing overlaps with one
+// Many rows of a product are bound by the clock under load: 32,000 x 25,088 x 1,024 by 256 x 256 tiles takes 684-719 us
+// (from card to card), 2.29-2.40 POPS, with the matrix pipes busy in 55 % of the cycles at 2.05 GHz (zeros for operands and no
+// traffic: 447 us where this took 712).  At k = 1,024 (to bf16, 47-56 us) the stores and the 64-bit epilogue, which nothing overlaps with one
 // workgroup a CU, take the larger part; 2,000 x 12,544 x 1,024 by 128 x 128 in two splits takes 38 us and 9 to join.
 // Tried: 32 x 32 x 32 instructions 711 -> 744 us; 128 x 256 tiles in a ring of three stages, two workgroups a CU,
 // 688 -> 874 us (45 -> 50 at k = 1,024); 128 x 128 a wave spills.
@@ -405,8 +405,8 @@ __global__ void __launch_bounds__(64) linear_i8_grad_join_kernel(const LiArgs A,
 // One launch from float rows (or codes) to the result: a workgroup takes LF_N output channels and all of k.  A thread owns
 // the 16-byte chunks t, t + 1024, ... of k, of the weight rows and of x alike, so that it needs nothing of its neighbours but
 // the row's maximum and the final sum; the weights, which are all there is to read, stay in its registers for every row of
-// x.  Each workgroup quantises x for itself, out of the L2.  One row of 12,544 by 1,024 channels: 6.4 us for 12.9 MB
-// (2.0 TB/s); a chain of load, maximum over the workgroup, codes and sum over the workgroup bounds it.
+// x.  Each workgroup quantises x for itself, out of the L2.  One row of 12,544 by 1,024 channels: 6.2 us for 12.9 MB
+// (2.1 TB/s); a chain of load, maximum over the workgroup, codes and sum over the workgroup bounds it.
 #define LF_THREADS 1024
 #define LF_N 4
 #define LF_CHUNKS 2 // of a thread: k up to 32,768
@@ -691,8 +691,8 @@ struct LiPlan {
 
 // k in `want` parts, as many as come out even, down to `least` stages each; not at all up to `whole` stages.
 // LI_SMALL: the tiles of 64.  One launch fewer is worth a few stages one after the other: 99 rows of 2,048 by 1,024 channels
-// whole : in four parts 12.3 : 11.3 us on the GPU, 13.2 : 17.1 us a call; the gradients of 512 x 1,024 x 1,024 26.2 : 32.3 us
-// on the GPU.
+// whole : in four parts 12.3 : 11.3 us on the GPU, 13.2 : 17.1 us a call; both gradients of 512 x 2,048 x 1,000 whole : in two
+// parts 39.5 : 42.2 us on the GPU, of 512 x 1,024 x 1,024 32.3 : 31.8.
 #define LI_SMALL 16, 32
 static LiPlan li_split(int bm, int bn, int M, int N, int K, int64_t want, int least = 8, int whole = 0)
 {
@@ -711,7 +711,7 @@ static LiPlan li_split(int bm, int bn, int M, int N, int K, int64_t want, int le
 }
 
 // Up to 256 rows: 64 x 64 tiles (32 x 64 up to 32 rows), k split over the CUs; they need half as many splits as larger ones
-// (99 rows of 12,544 13.2 us : 18.7).  Above, 128 x 128 or 256 x 256 by an estimate of the time, in ns:
+// (product and join of 99 rows of 12,544, calls replayed in a graph, 13.2 us : 18.7).  Above, 128 x 128 or 256 x 256 by an estimate of the time, in ns:
 //   256 x 256, one workgroup a CU: 870 a stage with the whole chip at it (there the clock gives way: 2.3 POPS), 700 at least;
 //   128 x 128: 320 a stage for each workgroup of a CU (1.6 POPS);
 //   and for a split k the sums' way out and back, at 8 TB/s, and a launch.
@@ -830,8 +830,8 @@ static bool li_shape_ok(int M, int N, int K)
 }
 static bool li_ws_ok(const void *ws) { return ((uintptr_t)ws & 255) == 0; }
 
-// The few-rows form.  1,024 channels, rows of 12,544: 1 / 2 / 3 / 4 rows 5.5 / 8.6 / 11.9 / 15.2 us against 14.5 by tiles and
-// three launches, which cost the host 6 us more than one.
+// The few-rows form.  1,024 channels, rows of 12,544, calls replayed in a graph: 1 / 2 / 3 / 4 rows 5.9 / 9.0 / 12.1 / 15.6 us
+// against 14.8 (five rows) by tiles and three launches, which cost the host 6 us more than one.
 static bool lf_takes(int M, int K) { return M <= 4 && K <= LF_THREADS * LF_CHUNKS * 16; }
 
 // The short-rows form (K >= 16: the last weight is read by a 16-byte load).  It reads the weights once per BM rows, so it

@@ -238,7 +238,7 @@ __device__ __forceinline__ void rap_stage_planes(float4 *s_plane, const float *_
 
 // What bounds this kernel (A/B builds on MI355X, batch 16 x 2000 RoIs, C = 512; DESIGN.md has the
 // table): the OUTPUT STORE STREAM.  With the arithmetic removed the stores alone take 0.77 ms of
-// the 0.91 ms; the arithmetic alone (LDS taps + packed FMAs + per-item set-up) takes 0.66 ms and
+// the 0.91 ms; the arithmetic alone (LDS taps + FMAs, packed ones at the time, + per-item set-up) takes 0.66 ms and
 // overlaps with them only in part.  How the 3.2 GB are handed to the memory system matters more
 // than anything computed here: the same bytes written as 64-item slices that straddle RoIs took
 // 1.07 ms, as whole (RoI, chunk) pieces per wave 0.77 ms (tools/store_probe.hip), and with the

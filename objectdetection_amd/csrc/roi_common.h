@@ -130,7 +130,7 @@ __device__ __forceinline__ RoiWindow roi_window(float4 rec, int H, int W, int nw
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// acc += w * f for four channels as two packed fp32 FMAs (v_pk_fma_f32).
+// acc += w * f for four channels, two at a time.  (The build keeps packed fp32 instructions off: these are four v_fma_f32.)
 __device__ __forceinline__ void pk_axpy4(f32x2 &lo, f32x2 &hi, float w, const float4 &f)
 {
     f32x2 w2 = {w, w};
