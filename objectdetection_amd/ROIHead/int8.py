@@ -21,28 +21,35 @@ class Int8TrainingLinear(Linear):
         return ops.LinearI8.apply(x, self.weight, self.bias, False)
 
 
-def follow(layers, int8):
-    """A head's own layers take the class of its choice, which may come later than they (set on a finished module, or one
-    pickled before it): the two classes hold the same."""
-    for layer in layers:
-        if type(layer) is (Linear if int8 else Int8TrainingLinear):
-            layer.__class__ = Int8TrainingLinear if int8 else Linear
-
-
 def fuses(layer):
-    """Whether a caller may compute this layer together with what follows: not where someone watches or changes what goes in
-    and out (hooks; weight normalisation as a pre-hook is one), nor a layer put in its place."""
-    return isinstance(layer, Int8TrainingLinear) and not (
+    """Whether a head may compute this layer together with what follows: not where someone watches or changes what goes in
+    and out (hooks; weight normalisation as a pre-hook is one), nor another kind of layer put in its place."""
+    return (isinstance(layer, Int8TrainingLinear) or type(layer) is Linear) and not (
         layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks or layer._backward_pre_hooks
         or _module._global_forward_hooks or _module._global_forward_pre_hooks or _module._global_backward_hooks
         or _module._global_backward_pre_hooks)
 
 
+def dense(layer, x):
+    """layer(x) in 8-bit integers.  A plain Linear (of a head built, or pickled, before it was set to int8) takes the class
+    that computes so, which holds the same."""
+    if type(layer) is Linear:
+        layer.__class__ = Int8TrainingLinear
+    return layer(x)
+
+
 def dense_relu(layer, x):
-    """relu(layer(x)), in one call where nothing needs the layer's own output."""
+    """relu(layer(x)) in 8-bit integers, in one call where nothing needs the layer's own output."""
     if fuses(layer):
         return ops.LinearI8.apply(x, layer.weight, layer.bias, True)
-    return functional.relu(layer(x))
+    return functional.relu(dense(layer, x))
+
+
+def as_float(layer):
+    """The layer of a head that is not, or no longer, set to int8."""
+    if type(layer) is Int8TrainingLinear:
+        layer.__class__ = Linear
+    return layer
 
 
 class Int8Linear(Module):

@@ -2,7 +2,7 @@
 train with straight-through gradients (ops.LinearI8); Int8TwoMLPHead serves what either has learnt."""
 from torch.nn import Linear, Module, functional
 
-from .int8 import Int8TrainingLinear, dense_relu, follow
+from .int8 import Int8TrainingLinear, as_float, dense_relu
 
 
 class TwoMLPHead(Module):
@@ -17,9 +17,8 @@ class TwoMLPHead(Module):
 
     def forward(self, x):
         x = x.flatten(start_dim=1)
-        follow((self.fc1, self.fc2), self.int8)
         if self.int8:
             return dense_relu(self.fc2, dense_relu(self.fc1, x))
-        x = functional.relu(self.fc1(x))
-        x = functional.relu(self.fc2(x))
+        x = functional.relu(as_float(self.fc1)(x))
+        x = functional.relu(as_float(self.fc2)(x))
         return x

@@ -5,7 +5,7 @@ import torch
 from torch.nn import Linear, Module
 
 from .. import ops
-from .int8 import Int8TrainingLinear, follow, fuses
+from .int8 import Int8TrainingLinear, as_float, dense, fuses
 
 
 class FasterRCNNPredictor(Module):
@@ -20,10 +20,11 @@ class FasterRCNNPredictor(Module):
 
     def forward(self, x):
         x = x.flatten(start_dim=1)
-        follow((self.cls_score, self.bbox_pred), self.int8)
-        if self.int8 and fuses(self.cls_score) and fuses(self.bbox_pred) and self.cls_score.bias is not None \
+        if not self.int8:
+            return as_float(self.cls_score)(x), as_float(self.bbox_pred)(x)
+        if fuses(self.cls_score) and fuses(self.bbox_pred) and self.cls_score.bias is not None \
                 and self.bbox_pred.bias is not None:  # one product: x is quantised once
             y = ops.LinearI8.apply(x, torch.cat([self.cls_score.weight, self.bbox_pred.weight]),
                                    torch.cat([self.cls_score.bias, self.bbox_pred.bias]), False)
             return y[:, :self.cls_score.out_features], y[:, self.cls_score.out_features:]
-        return self.cls_score(x), self.bbox_pred(x)
+        return dense(self.cls_score, x), dense(self.bbox_pred, x)

@@ -280,6 +280,7 @@ def test_layers_follow_a_choice_made_late():
             other.int8 = True
             with pytest.raises(_lib.FrcnnError):  # the 8-bit layers have no CPU form
                 other(x)
+            assert all(type(layer) is torch.nn.Linear for layer in other.children())  # they may be another module's too
             for layer in list(other.children()):
                 layer.register_forward_hook(lambda m, i, o: None)
             with pytest.raises(_lib.FrcnnError):
